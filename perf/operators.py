@@ -167,7 +167,7 @@ def _cu(lens):
 def _tree(seed, lens, tokens, tree):
     """Bit masks (rows, words) of each drafted token's path: itself and its ancestors, parents drawn at random."""
     words = (tokens + 63) // 64
-    rs = np.random.RandomState(seed * 31 + 5)
+    rs = np.random.RandomState((seed * 31 + 5) % 2 ** 32)
     mask = np.zeros((len(lens) * tokens, words), dtype=np.uint64)
     for b in range(len(lens)):
         for i in range(tokens):
@@ -249,7 +249,7 @@ def prepare(case, seed):
         s["roots"], s["prompt"] = s["slots"][:batch].clone(), cache.seqlens[:batch].clone()
         s["beams"] = torch.cat([s["children"], s["roots"]])         # a parent comes last and keeps its own page
     else:
-        rs = np.random.RandomState(seed * 13 + 1)
+        rs = np.random.RandomState((seed * 13 + 1) % 2 ** 32)
         most = max(1, t // 4)
         keep = np.stack([np.sort(rs.permutation(t)[:most]) for _ in range(batch)]).astype(np.int32)
         s.update(keep=torch.from_numpy(keep).to(DEV), cu=_cu([t] * batch), lens=cache.seqlens.clone(),
