@@ -31,7 +31,8 @@ if _PROBE_FLAGS and ("-DFA_AB_PROBE_BUILD" not in EXTRA_CFLAGS or OUT == DEFAULT
                      "build it only with -DFA_AB_PROBE_BUILD and FA_BUILD_OUT set to a variant library")
 
 KERNEL_TUS = ["fa_d32_fwd.hip", "fa_d64_fwd.hip", "fa_d128_fwd.hip", "fa_d32_bwd.hip", "fa_d64_bwd.hip", "fa_d128_bwd.hip"]
-SOURCES = ["fa_api.cpp", "fa_asm.cpp", "fa_aux.hip", "fa_padding.hip", "fa_rotary.hip"] + KERNEL_TUS
+WINDOW_TUS = ["fa_window_d32.hip", "fa_window_d64.hip", "fa_window_d128.hip"]
+SOURCES = ["fa_api.cpp", "fa_asm.cpp", "fa_aux.hip", "fa_padding.hip", "fa_rotary.hip", "fa_window_api.cpp", "fa_cache.hip"] + KERNEL_TUS + WINDOW_TUS
 # hand-scheduled assembly kernels: generator script -> .s -> code object -> embedded byte array
 ASM_GEN = os.path.join(CSRC, "asm", "gen_fwd.py")
 # (dtype, head-dim tile, waves per workgroup or "p" = the persistent 4-wave form, symbol)
@@ -54,6 +55,10 @@ SOURCE_FLAGS = {
     "fa_d32_fwd.hip": _TRACKERS, "fa_d64_fwd.hip": _TRACKERS, "fa_d128_fwd.hip": _TRACKERS,
     "fa_d32_bwd.hip": _ITILP, "fa_d128_bwd.hip": _ITILP,
 }
+# no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on this part
+_NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+for _src in WINDOW_TUS + ["fa_window_api.cpp", "fa_cache.hip"]:
+    SOURCE_FLAGS[_src] = SOURCE_FLAGS.get(_src, []) + _NO_PACKED_FP32
 ARCH = os.environ.get("FA_OFFLOAD_ARCH", "gfx950")
 
 
@@ -79,7 +84,7 @@ def _newer(target, deps):
 
 def _deps():
     hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
-    hdrs.append(os.path.join(INCLUDE, "fa_hip.h"))
+    hdrs += [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE) if f.endswith(".h")]
     return hdrs + [os.path.abspath(__file__)]
 
 
@@ -140,28 +145,40 @@ def compile_blob(blob_cpp, force=False):
     return obj
 
 
-TORCH_EXT_SRC = os.path.join(CSRC, "fa_torch.cpp")
+TORCH_EXT_SRCS = [os.path.join(CSRC, "fa_torch.cpp"), os.path.join(CSRC, "fa_torch_window.cpp")]
 TORCH_EXT_OUT = os.path.join(HERE, "flash_attn", "_fa_C.so")
 
 
 def build_torch_ext(force=False):
-    """The compiled fwd/bwd binding (csrc/fa_torch.cpp): a host-only pybind11 module over the C ABI,
+    """The compiled binding (csrc/fa_torch.cpp, csrc/fa_torch_window.cpp): a host-only pybind11 module over the C ABI,
     linked against the in-tree libfa_hip.so (rpath $ORIGIN) and torch's libraries."""
-    deps = [TORCH_EXT_SRC, os.path.join(INCLUDE, "fa_hip.h"), OUT, os.path.abspath(__file__)]
+    deps = TORCH_EXT_SRCS + [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)] + [OUT, os.path.abspath(__file__)]
     if not force and _newer(TORCH_EXT_OUT, deps):
         return TORCH_EXT_OUT
     import sysconfig
     import torch
     tdir = os.path.dirname(torch.__file__)
     abi = int(getattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", True))
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_fa_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
-           "-I", os.path.join(tdir, "include"), "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-           "-I", sysconfig.get_paths()["include"], "-I", "/opt/rocm/include", "-I", INCLUDE,
-           TORCH_EXT_SRC, "-o", TORCH_EXT_OUT,
+    flags = ["-O2", "-std=c++17", "-fPIC",
+             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_fa_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+             "-I", os.path.join(tdir, "include"), "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
+             "-I", sysconfig.get_paths()["include"], "-I", "/opt/rocm/include", "-I", INCLUDE]
+    cxx = os.environ.get("CXX", "g++")
+    os.makedirs(BUILD, exist_ok=True)
+
+    def compile_src(src):
+        obj = os.path.join(BUILD, os.path.basename(src) + ".o")
+        hdrs = [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
+        if force or not _newer(obj, [src, os.path.abspath(__file__)] + hdrs):
+            _run([cxx] + flags + ["-c", src, "-o", obj])
+        return obj
+
+    with cf.ThreadPoolExecutor(max_workers=len(TORCH_EXT_SRCS)) as ex:
+        objs = list(ex.map(compile_src, TORCH_EXT_SRCS))
+    cmd = ([cxx, "-shared"] + objs + ["-o", TORCH_EXT_OUT,
            "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-           "-L", os.path.dirname(OUT), "-l:libfa_hip.so", "-Wl,-rpath,$ORIGIN"]
+           "-L", os.path.dirname(OUT), "-l:libfa_hip.so", "-Wl,-rpath,$ORIGIN"])
     _run(cmd)
     return TORCH_EXT_OUT
 

@@ -16,6 +16,7 @@
 #include <string>
 
 #include "fa_launch.h"
+#include "fa_window_launch.h"
 
 namespace {
 
@@ -68,6 +69,20 @@ int check_common(const Args *a, const char *fn) {
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
+
+// the same error text for the other files of the C ABI (fa_window_launch.h)
+namespace fa {
+int set_error(int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
+}
+void clear_error() { g_last_error.clear(); }
+}  // namespace fa
 
 extern "C" {
 

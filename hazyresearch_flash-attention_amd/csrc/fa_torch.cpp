@@ -596,6 +596,8 @@ struct IndexPutFirstAxisFn : public torch::autograd::Function<IndexPutFirstAxisF
 
 }  // namespace
 
+void bind_window(pybind11::module &m);   // fa_torch_window.cpp
+
 PYBIND11_MODULE(_fa_C, m) {
     m.doc() = "compiled binding of libfa_hip.so (fwd / bwd over include/fa_hip.h)";
     m.def("fwd", &fwd, pybind11::arg("q"), pybind11::arg("k"), pybind11::arg("v"), pybind11::arg("cu_q"),
@@ -652,5 +654,6 @@ PYBIND11_MODULE(_fa_C, m) {
         if (!needs_grad({&values})) return pad_rows(values, indices, first_axis_dim);
         return IndexPutFirstAxisFn::apply(values, indices, first_axis_dim)[0];
     });
+    bind_window(m);
     m.def("version", [] { return std::string(fa_version()); });
 }

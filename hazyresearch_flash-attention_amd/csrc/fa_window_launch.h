@@ -1,0 +1,19 @@
+// fa_window_launch.h — launchers of the windowed and paged kernels, one translation unit per head-dim tile.
+#pragma once
+#include "fa_launch.h"
+#include "../../include/fa_window_hip.h"
+
+namespace fa {
+struct WinFwdArgs;
+struct WinBwdArgs;
+// `shape` of a forward launch: row waves x key groups x keys per tile
+enum WinShape { WIN_4X1X64 = 0, WIN_2X2X32 = 1, WIN_1X4X32 = 2 };
+int win_shape_rows(WinShape s);      // packed rows per workgroup
+int win_shape_groups(WinShape s);
+int win_shape_keys(WinShape s);      // keys per tile
+template <int D> hipError_t launch_window_fwd(const WinFwdArgs &a, int dtype, bool paged, WinShape shape, hipStream_t s);
+template <int D> hipError_t launch_window_bwd(const WinBwdArgs &a, int dtype, int max_rows, int max_k, hipStream_t s);
+// the error text of the C ABI (fa_api.cpp)
+int set_error(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+void clear_error();
+}  // namespace fa
