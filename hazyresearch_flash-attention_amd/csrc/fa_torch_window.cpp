@@ -136,7 +136,7 @@ std::vector<at::Tensor> window_bwd(const at::Tensor &dout_, const at::Tensor &q_
     c10::DeviceGuard guard(q_.device());
     const at::Tensor q = rows(q_), k = rows(k_), v = rows(v_), dout = rows(dout_);
     const auto dense = [](const at::Tensor &t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); };
-    at::Tensor dq = dense(q), dk = dense(k), dv = dense(v), d = at::empty_like(lse);
+    at::Tensor dq = dense(q), dk = dense(k), dv = dense(v);
     if (max_q == 0) dq.zero_();
     if (max_k == 0) {
         dk.zero_();
@@ -147,7 +147,6 @@ std::vector<at::Tensor> window_bwd(const at::Tensor &dout_, const at::Tensor &q_
     a.dq = dq.data_ptr();
     a.dk = dk.data_ptr();
     a.dv = dv.data_ptr();
-    a.softmax_d = d.data_ptr<float>();
     a.do_row_stride = dout.stride(0); a.do_head_stride = dout.stride(1);
     a.dq_row_stride = dq.stride(0); a.dq_head_stride = dq.stride(1);
     a.dk_row_stride = dk.stride(0); a.dk_head_stride = dk.stride(1);

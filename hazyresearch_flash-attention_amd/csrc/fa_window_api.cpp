@@ -21,8 +21,19 @@ namespace {
 constexpr int NO_WINDOW = 0x3FFFFFFF;      // more than any position (lengths are below 2^30)
 constexpr int64_t LEN_LIMIT = 1 << 30;
 
-bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 int tile_of(int head_dim) { return head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : 128; }
+
+// block_order's `order` (fa_window_common.h). A group's K/V (the keys in view of its heads) stay below 8 MiB, twice
+// an XCD's L2: 8 x 2048 tokens, 12 heads of 64, no window: groups of 12 dkv 163 us, of 8 173, of 1 198.
+int order_for(int64_t pairs, int64_t window, int64_t max_k, int head_dim) {
+    const int64_t keys = window < max_k ? window : max_k;
+    if (pairs % 8 == 0) {
+        const int64_t one = (keys > 64 ? keys : 64) * tile_of(head_dim) * 4, g = ((int64_t)8 << 20) / one;
+        return (int)(g < 1 ? 1 : (g > pairs / 8 ? pairs / 8 : g));
+    }
+    return 2 * keys <= max_k ? 0 : -1;
+}
+bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // what both entry families ask of the sizes
 int check_sizes(const char *fn, int batch, int nheads, int nheads_k, int head_dim, int max_q, int window, int sinks,
@@ -77,7 +88,6 @@ int check_window(const FaWindowArgs *a, const char *fn, bool bwd) {
         if ((rc = check_rows(fn, "v", a->v, a->v_row_stride, a->v_head_stride, a->nheads_k, d))) return rc;
     }
     if (bwd && has_q) {
-        if (!a->softmax_d) return set_error(FA_ERR_INVALID_ARGUMENT, "%s: softmax_d is NULL", fn);
         if ((rc = check_rows(fn, "dout", a->dout, a->do_row_stride, a->do_head_stride, a->nheads, d))) return rc;
         if ((rc = check_rows(fn, "dq", a->dq, a->dq_row_stride, a->dq_head_stride, a->nheads, d))) return rc;
     }
@@ -166,6 +176,46 @@ PagedPlan plan_paged(const FaPagedArgs *a) {
     return p;
 }
 
+// The backward's shape, its workspace laid out behind `ws`, and the bytes it takes.
+//
+// The sinks' rows behind the window get workgroups of their own when a sequence may be longer than two windows:
+// shares of 1024 rows (512 where a block of keys itself walks more than 4096 rows, so that they do not add a round of
+// their own: 292 us against 311 at 8192 tokens, window 1024, 16 heads on 4; at 2048 tokens, window 256, 12 heads 1024
+// rows take 71 us, 512 75), 64 to a head at most and no more than the partial sums' WIN_SINK_BYTES allow.
+constexpr int64_t WIN_SINK_BYTES = (int64_t)64 << 20;
+WinBwdPlan plan_bwd(const FaWindowArgs *a, WinBwdArgs &w, char *ws, int64_t &bytes) {
+    WinBwdPlan p{};
+    const int group = a->nheads / a->nheads_k;
+    p.max_rows = a->total_q > 0 ? a->max_seqlen_q * group : 0;
+    p.max_k = a->total_k > 0 ? a->max_seqlen_k : 0;
+    const int64_t window = a->window > 0 && a->window < NO_WINDOW ? a->window : NO_WINDOW;
+    w.window = (int)window;
+    p.order = order_for((int64_t)a->nheads_k * a->batch, window, p.max_k, a->head_dim);
+    w.sinks = a->num_sinks < p.max_k ? a->num_sinks : p.max_k;
+    w.chunks = w.sink_blocks = w.per_chunk = w.slots = 0;
+    bytes = a->total_q * a->nheads * (int64_t)sizeof(f32x2);
+    bytes = (bytes + 255) / 256 * 256;
+    w.ws_rows = (f32x2 *)ws;
+    if (w.sinks > 0 && p.max_rows > 0 && p.max_k > 2 * window) {
+        const int64_t part = (int64_t)a->batch * a->nheads_k * w.sinks * 2 * tile_of(a->head_dim) * (int64_t)sizeof(float);
+        const int64_t share = (window + 32 * WIN_DKV_BLOCKS) * group > 4096 ? 512 : 1024;
+        int64_t chunks = (p.max_rows + share - 1) / share;
+        const int64_t fit = (WIN_SINK_BYTES / part - 1) / WIN_DKV_BLOCKS;
+        chunks = chunks < fit ? chunks : fit;
+        chunks = chunks < 1 ? 1 : (chunks > 64 ? 64 : chunks);
+        const int64_t per = ((p.max_rows + chunks - 1) / chunks + 31) / 32 * 32;
+        w.per_chunk = (int)per;
+        w.chunks = (int)((p.max_rows + per - 1) / per);
+        w.sink_blocks = (w.sinks + 31) / 32;
+        w.slots = w.chunks * WIN_DKV_BLOCKS + 1;
+        w.dchunks = Div::of(w.chunks);
+        w.dsinkb = Div::of(w.sink_blocks);
+        w.ws_part = (float *)(ws + bytes);
+        bytes += part * w.slots;
+    }
+    return p;
+}
+
 int64_t paged_bytes(const FaPagedArgs *a, const PagedPlan &p) {
     if (p.nsplit == 1) return 0;
     const int64_t rows = (int64_t)p.nsplit * a->total_q * a->nheads;
@@ -198,8 +248,12 @@ int fa_window_fwd(const FaWindowArgs *a, void *stream) {
     w.lse_stride = a->lse_stride;
     w.window = a->window > 0 && a->window < NO_WINDOW ? a->window : NO_WINDOW;
     w.sinks = a->num_sinks;
-    w.nrb = (int)(((int64_t)a->max_seqlen_q * w.group + 127) / 128);
+    w.nrb = (int)(((int64_t)a->max_seqlen_q * w.group + 32 * WIN_FWD_WAVES - 1) / (32 * WIN_FWD_WAVES));
     w.nsplit = 1;
+    w.dgroup = Div::of(w.group);
+    w.dheads = Div::of(w.nheads_k);
+    w.dsplit = Div::of(1);
+    w.order = BlockOrder::of(w.nrb, w.nheads_k * w.batch, order_for((int64_t)w.nheads_k * w.batch, w.window, a->max_seqlen_k, a->head_dim));
     w.scale = a->softmax_scale;
     if ((rc = grid_ok("fa_window_fwd", (int64_t)w.nrb * w.nheads_k * w.batch))) return rc;
     hipStream_t s = (hipStream_t)stream;
@@ -215,7 +269,16 @@ int fa_window_fwd(const FaWindowArgs *a, void *stream) {
 int64_t fa_window_bwd_workspace(const FaWindowArgs *a) {
     clear_error();
     if (!a) return -set_error(FA_ERR_INVALID_ARGUMENT, "fa_window_bwd_workspace: args is NULL");
-    return 0;
+    const int rc = check_sizes("fa_window_bwd_workspace", a->batch, a->nheads, a->nheads_k, a->head_dim, a->max_seqlen_q,
+                               a->window, a->num_sinks, a->softmax_scale, a->dtype);
+    if (rc) return -rc;
+    if (a->total_q < 0 || a->total_k < 0 || a->max_seqlen_k < 0 ||
+        (a->total_q + a->total_k + a->max_seqlen_q) * (a->nheads / a->nheads_k) >= LEN_LIMIT)
+        return -set_error(FA_ERR_INVALID_ARGUMENT, "fa_window_bwd_workspace: lengths out of range");
+    WinBwdArgs w{};
+    int64_t bytes;
+    plan_bwd(a, w, nullptr, bytes);
+    return bytes;
 }
 
 int fa_window_bwd(const FaWindowArgs *a, void *stream) {
@@ -224,38 +287,35 @@ int fa_window_bwd(const FaWindowArgs *a, void *stream) {
     if (rc) return rc;
     WinBwdArgs w{};
     w.q = (const uint16_t *)a->q; w.k = (const uint16_t *)a->k; w.v = (const uint16_t *)a->v;
-    w.dout = (const uint16_t *)a->dout; w.lse = a->softmax_lse; w.delta = a->softmax_d;
+    w.o = (const uint16_t *)a->o; w.dout = (const uint16_t *)a->dout; w.lse = a->softmax_lse;
     w.dq = (uint16_t *)a->dq; w.dk = (uint16_t *)a->dk; w.dv = (uint16_t *)a->dv;
     w.cu_q = a->cu_seqlens_q; w.cu_k = a->cu_seqlens_k;
     w.q_rs = a->q_row_stride; w.q_hs = a->q_head_stride; w.k_rs = a->k_row_stride; w.k_hs = a->k_head_stride;
-    w.v_rs = a->v_row_stride; w.v_hs = a->v_head_stride; w.do_rs = a->do_row_stride; w.do_hs = a->do_head_stride;
+    w.v_rs = a->v_row_stride; w.v_hs = a->v_head_stride; w.o_rs = a->o_row_stride; w.o_hs = a->o_head_stride;
+    w.do_rs = a->do_row_stride; w.do_hs = a->do_head_stride;
     w.dq_rs = a->dq_row_stride; w.dq_hs = a->dq_head_stride; w.dk_rs = a->dk_row_stride; w.dk_hs = a->dk_head_stride;
     w.dv_rs = a->dv_row_stride; w.dv_hs = a->dv_head_stride;
     w.total_q = a->total_q; w.total_k = a->total_k;
     w.batch = a->batch; w.nheads = a->nheads; w.nheads_k = a->nheads_k; w.head_dim = a->head_dim;
     w.group = a->nheads / a->nheads_k;
+    w.dgroup = Div::of(w.group);
+    w.dheads = Div::of(w.nheads_k);
     w.lse_stride = a->lse_stride;
-    w.window = a->window > 0 && a->window < NO_WINDOW ? a->window : NO_WINDOW;
-    w.sinks = a->num_sinks;
     w.scale = a->softmax_scale;
-    const int max_rows = a->total_q > 0 ? a->max_seqlen_q * w.group : 0, max_k = a->total_k > 0 ? a->max_seqlen_k : 0;
-    if ((rc = grid_ok("fa_window_bwd", ((int64_t)(max_rows > max_k ? max_rows : max_k) / 32 + 1) * w.nheads_k * w.batch))) return rc;
+    int64_t bytes;
+    const WinBwdPlan p = plan_bwd(a, w, (char *)a->workspace, bytes);
+    if (bytes > 0 && (!a->workspace || !al16(a->workspace) || a->workspace_bytes < bytes))
+        return set_error(FA_ERR_INVALID_ARGUMENT, "fa_window_bwd: workspace of %lld bytes needed", (long long)bytes);
+    const int64_t most = (int64_t)(p.max_rows > p.max_k ? p.max_rows : p.max_k) / 32 + 1 + (int64_t)w.chunks * w.sink_blocks;
+    if ((rc = grid_ok("fa_window_bwd", most * w.nheads_k * w.batch))) return rc;
+    if (w.chunks > 0 && (int64_t)w.nheads_k * w.batch > 65535)
+        return set_error(FA_ERR_UNSUPPORTED, "fa_window_bwd: batch * nheads_k above 65535");
     hipStream_t s = (hipStream_t)stream;
-    hipError_t e = hipSuccess;
-    if (max_rows > 0) {
-        FaBwdArgs d{};      // delta = rowsum(dO * O): the dense backward's first pass, dq_accum unused
-        d.dout = a->dout; d.out = a->o; d.softmax_d = a->softmax_d; d.cu_seqlens_q = a->cu_seqlens_q;
-        d.do_row_stride = a->do_row_stride; d.do_head_stride = a->do_head_stride;
-        d.o_row_stride = a->o_row_stride; d.o_head_stride = a->o_head_stride;
-        d.batch = a->batch; d.nheads = a->nheads; d.head_dim = a->head_dim; d.max_seqlen_q = a->max_seqlen_q;
-        d.total_q = (int32_t)a->total_q; d.lse_stride = a->lse_stride; d.dtype = a->dtype;
-        e = launch_bwd_pre(d, s);
-        if (e != hipSuccess) return hip_rc(e, "fa_window_bwd delta launch");
-    }
+    hipError_t e;
     switch (tile_of(a->head_dim)) {
-        case 32: e = launch_window_bwd<32>(w, a->dtype, max_rows, max_k, s); break;
-        case 64: e = launch_window_bwd<64>(w, a->dtype, max_rows, max_k, s); break;
-        default: e = launch_window_bwd<128>(w, a->dtype, max_rows, max_k, s); break;
+        case 32: e = launch_window_bwd<32>(w, a->dtype, p, s); break;
+        case 64: e = launch_window_bwd<64>(w, a->dtype, p, s); break;
+        default: e = launch_window_bwd<128>(w, a->dtype, p, s); break;
     }
     return hip_rc(e, "fa_window_bwd launch");
 }
@@ -294,6 +354,10 @@ int fa_paged_fwd(const FaPagedArgs *a, void *stream) {
     w.window = a->window > 0 && a->window < NO_WINDOW ? a->window : NO_WINDOW;
     w.sinks = a->num_sinks;
     w.nrb = p.nrb; w.nsplit = p.nsplit;
+    w.dgroup = Div::of(w.group);
+    w.dheads = Div::of(w.nheads_k);
+    w.dsplit = Div::of(w.nsplit);
+    w.order.blk = Div::of(w.nrb);
     w.scale = a->softmax_scale;
     if (p.nsplit > 1) {
         w.ws_o = (float *)a->workspace;

@@ -2,29 +2,47 @@
 //
 // With P = exp(scale Q K^T - lse) on the entries a row sees and 0 elsewhere, delta = rowsum(dO * O):
 //     dP = dO V^T,  dS = P (dP - delta),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,
-// dK and dV summed over the query heads of a group. Two kernels, each writing its outputs once, in one order, with
-// no atomics: dQ by query rows (the forward's walk), dK and dV by keys. S and dP are computed in both: 7 matrix
-// products of the forward's size against 5 with dQ by fp32 atomics, whose order changes the result and whose
-// rate bounds it (1.3 TB/s measured for the dense backward).
+// dK and dV summed over the query heads of a group. dQ is computed by query rows (the forward's walk), dK and dV by
+// keys, each written once, in one order, with no atomics. S and dP are computed in both: 7 matrix products of the
+// forward's size against 5 with dQ by fp32 atomics, whose order changes the result and whose rate bounds it
+// (1.3 TB/s measured for the dense backward).
+//
+// Row constants: ws_rows[i] = {lse log2(e), -delta} of packed row i of a sequence and key/value head, rows of a
+// head one after the other, so that a tile's 32 pairs are 256 contiguous bytes (one LDS-DMA of 4 bytes a lane).
+// The dQ kernel leaves them for the dK, dV kernel. delta comes from O in 16 bits, whose rounding is lost among many
+// keys but shows where a row sees few; there it is summed from P and dP in fp32 first (WIN_EXACT_TILES).
 #pragma once
 
 #include "fa_window_common.h"
 
 namespace fa {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 struct WinBwdArgs {
-    const uint16_t *q, *k, *v, *dout;
-    const float *lse, *delta;
+    const uint16_t *q, *k, *v, *o, *dout;
+    const float *lse;
     uint16_t *dq, *dk, *dv;
-    float *ws;
+    f32x2 *ws_rows;               // [total_q * nheads]
+    float *ws_part;               // [batch * nheads_k][sinks][slots][2][D]: dK, dV of the sinks by parts
     const int32_t *cu_q, *cu_k;
-    int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, do_rs, do_hs;
+    int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, o_rs, o_hs, do_rs, do_hs;
     int64_t dq_rs, dq_hs, dk_rs, dk_hs, dv_rs, dv_hs;
     int64_t total_q, total_k;
     int batch, nheads, nheads_k, head_dim, group;
-    int lse_stride, window, sinks, nblk;
+    int lse_stride, window, sinks;
+    // the sinks' rows behind the window, cut into `chunks` shares (0: walked with the rest): blocks of 32 keys,
+    // partial sums a share leaves (one for each wave or pair), `slots` of them in all and the window's own
+    int chunks, sink_blocks, per_chunk, slots;
     float scale;
+    Div dgroup, dheads, dchunks, dsinkb;      // by group, nheads_k, chunks, sink_blocks
+    BlockOrder order;
 };
+
+// first packed row (of the whole tensor's row constants) of a sequence and key/value head
+__device__ __forceinline__ int64_t rows_base(const WinBwdArgs &a, int q_start, int sq, int kvh) {
+    return (int64_t)q_start * a.nheads + (int64_t)kvh * sq * a.group;
+}
 
 // ---------------------------------------------------------------------------------------------- dQ
 template <int D, int NW>
@@ -43,6 +61,11 @@ struct WinDqCfg {
 // A wave owns 32 packed query rows (lane = row): S^T = K Q^T and dP^T = V dO^T with Q and dO rows in registers,
 // dS^T packed in place is the B operand of dQ^T += K^T dS^T (K^T by transposed LDS reads). lse and delta are per
 // lane, so no exchange between rows at all.
+//
+// A workgroup of few tiles walks them twice, first for delta = sum_j P_j dP_j: with the 16-bit O's delta the error of
+// dQ and dK (rms, 60 to 400 keys from the sequence's start) measured 1.5 to 1.65 times that of a 32-bit backward
+// rounded once, with this one 1.4 to 1.45 (what the rounding of dS leaves). 2 of 5 products more on those tiles.
+constexpr int WIN_EXACT_TILES = 4;
 template <int D, typename T, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdArgs a) {
     using C = WinDqCfg<D, NW>;
@@ -50,18 +73,19 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
     constexpr float LOG2E = 1.4426950408889634f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
-    zero_tail(a.dq, a.dq_rs, a.dq_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
-    int w = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int rb = a.nblk - 1 - w % a.nblk;
-    w /= a.nblk;
-    const int kvh = w % a.nheads_k;
-    const int b = w / a.nheads_k;
+    int rb, w;
+    a.order.get(blockIdx.x, rb, w);
+    const int b = a.dheads.div(w);
+    const int kvh = w - b * a.nheads_k;
     int q_start, sq, k_start, klen;
     seq_bounds(a.cu_q, b, a.total_q, q_start, sq);
     seq_bounds(a.cu_k, b, a.total_k, k_start, klen);
     const int off = klen - sq;
     const int G = a.group, R = sq * G, r0 = rb * C::BM;
-    if (r0 >= R) return;
+    if (r0 >= R) {
+        zero_tail(a.dq, a.dq_rs, a.dq_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
+        return;
+    }
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -69,33 +93,13 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
     const int head_dim = a.head_dim;
     const int rw = r0 + 32 * wave, row = rw + l32;
     const int rc = row < R ? row : R - 1;
-    const int t = rc / G, g = rc - t * G, h = kvh * G + g;
+    const int t = a.dgroup.div(rc), g = rc - t * G, h = kvh * G + g;
     const int pos = off + t;
-    int pmin = off + rw / G, pmax = off + (rw + 31 < R ? rw + 31 : R - 1) / G;
+    int pmin = off + a.dgroup.div(rw), pmax = off + a.dgroup.div(rw + 31 < R ? rw + 31 : R - 1);
     if (rw >= R) pmin = pmax = pos;
-    int k_end = off + (r0 + C::BM < R ? r0 + C::BM - 1 : R - 1) / G + 1;
+    int k_end = off + a.dgroup.div(r0 + C::BM < R ? r0 + C::BM - 1 : R - 1) + 1;
     k_end = k_end < klen ? k_end : klen;
-    const TileWalk walk = tile_walk(off + r0 / G, k_end, a.window, a.sinks, C::BN);
-
-    typename T::frag qf[D / 16], df[D / 16];
-    {
-        const uint16_t *qp = a.q + (int64_t)(q_start + t) * a.q_rs + (int64_t)h * a.q_hs;
-        const uint16_t *dp = a.dout + (int64_t)(q_start + t) * a.do_rs + (int64_t)h * a.do_hs;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const int c = 2 * ks + hi;
-            u32x4 x = {0u, 0u, 0u, 0u}, y = {0u, 0u, 0u, 0u};
-            if (c * 8 < head_dim) {
-                x = gload128(qp + c * 8);
-                y = gload128(dp + c * 8);
-            }
-            qf[ks] = as_frag<T>(x);
-            df[ks] = as_frag<T>(y);
-        }
-    }
-    const int64_t li = (int64_t)(b * a.nheads + h) * a.lse_stride + t;
-    const float lse2 = a.lse[li] * LOG2E, delta = a.delta[li];
-    const float c_log2 = a.scale * LOG2E;
+    const TileWalk walk = tile_walk(off + a.dgroup.div(r0), k_end, a.window, a.sinks, C::BN);
 
     const uint16_t *kbase = a.k + (int64_t)k_start * a.k_rs + (int64_t)kvh * a.k_hs;
     const uint16_t *vbase = a.v + (int64_t)k_start * a.v_rs + (int64_t)kvh * a.v_hs;
@@ -124,23 +128,49 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
         }
     };
 
-    const int grp = (lane >> 4) & 1, qq = (lane & 15) >> 2, pp = lane & 3;
-    int k_rd[2][D / 16];
+    // the first tile is on its way before the rows are read
+    if (walk.n > 0) stage(0, 0);
+    typename T::frag qf[D / 16], df[D / 16];
+    float delta = 0.f;
+    {
+        const uint16_t *qp = a.q + (int64_t)(q_start + t) * a.q_rs + (int64_t)h * a.q_hs;
+        const uint16_t *dp = a.dout + (int64_t)(q_start + t) * a.do_rs + (int64_t)h * a.do_hs;
+        const uint16_t *op = a.o + (int64_t)(q_start + t) * a.o_rs + (int64_t)h * a.o_hs;
+        u32x4 x[D / 16], y[D / 16], z[D / 16];
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) k_rd[st][ks] = S::off(32 * st + l32, 2 * ks + hi);
-    int t_rd[D / 32][2][2][2];
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const int r = 32 * st + 16 * s2 + 4 * hi + qq, col = 32 * dt + 16 * grp + 4 * pp;
-                t_rd[dt][st][s2][0] = S::off8(r, col);
-                t_rd[dt][st][s2][1] = S::off8(r + 8, col);
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const int c = 2 * ks + hi;
+            x[ks] = y[ks] = z[ks] = u32x4{0u, 0u, 0u, 0u};
+            if (c * 8 < head_dim) {
+                x[ks] = gload128(qp + c * 8);
+                y[ks] = gload128(dp + c * 8);
+                z[ks] = gload128(op + c * 8);
             }
+        }
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            qf[ks] = as_frag<T>(x[ks]);
+            df[ks] = as_frag<T>(y[ks]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                delta += T::lo_float(y[ks][e]) * T::lo_float(z[ks][e]) + T::hi_float(y[ks][e]) * T::hi_float(z[ks][e]);
+        }
+        delta = pair_sum(delta);
+    }
+    const float lse2 = a.lse[(int64_t)(b * a.nheads + h) * a.lse_stride + t] * LOG2E;
+    const float c_log2 = a.scale * LOG2E;
+
+    const int grp = (lane >> 4) & 1, qq = (lane & 15) >> 2, pp = lane & 3;
+    int k_rd[D / 16];                 // rows 32 further on are an immediate offset (the swizzle goes by row % 16)
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) k_rd[ks] = S::off(l32, 2 * ks + hi);
+    int t_rd[D / 32][2];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+        const int r = 4 * hi + qq, col = 32 * dt + 16 * grp + 4 * pp;
+        t_rd[dt][0] = S::off8(r, col);
+        t_rd[dt][1] = S::off8(r + 8, col);
+    }
 
     f32x16 dq[D / 32];
 #pragma unroll
@@ -148,317 +178,562 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[dt][r] = 0.f;
 
-    auto compute = [&](int j0, int buf) __attribute__((always_inline)) {
+    // one tile, 32 keys at a time; SUM: delta's terms alone
+    float dsum = 0.f;
+    auto compute = [&](auto sum_tag, int j0, int buf) __attribute__((always_inline)) {
+        constexpr bool SUM = decltype(sum_tag)::value;
         const char *kb = smem + buf * C::TILE, *vb = smem + (2 + buf) * C::TILE;
-        typename T::frag pf[2][2];
-        // the mask runs in a copy of the sub-tile behind one wave-uniform branch: P and dS by selection, so that
-        // an infinity in a masked place (lse of a row that sees nothing) adds 0
-        auto sub = [&](auto masked_tag) __attribute__((always_inline)) {
-            constexpr bool MASKED = decltype(masked_tag)::value;
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                f32x16 s, dp;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = -delta; }
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    s = T::mfma32(as_frag<T>(lds_read128(kb, k_rd[st][ks])), qf[ks], s);
-                    dp = T::mfma32(as_frag<T>(lds_read128(vb, k_rd[st][ks])), df[ks], dp);
-                }
-                uint32_t m = 0;
-                if constexpr (MASKED) {
-                    const int j = j0 + 32 * st;
-                    m = (seen_bits(j, pos, a.window, a.sinks) & bits_below(klen - j)) >> (4 * hi);
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float x = fast_exp2(fmaf(s[r], c_log2, -lse2)) * dp[r];
-                    s[r] = MASKED && !(m & (1u << crow(r, 0))) ? 0.f : x;
-                }
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    u32x4 pk;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) pk[e] = T::pack2(s[8 * s2 + 2 * e], s[8 * s2 + 2 * e + 1]);
-                    pf[st][s2] = as_frag<T>(pk);
-                }
-            }
-        };
         const bool whole = j0 + C::BN - 1 <= pmin && (j0 > pmax - a.window || j0 + C::BN <= a.sinks) && j0 + C::BN <= klen;
-        if (__builtin_amdgcn_readfirstlane((int)whole))
-            sub(std::false_type{});
-        else
-            sub(std::true_type{});
+        const bool masked = !__builtin_amdgcn_readfirstlane((int)whole);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt)
+        for (int st = 0; st < 2; ++st) {
+            const int ro = 32 * st * S::ROW_BYTES;
+            f32x16 s, dp;
 #pragma unroll
-            for (int st = 0; st < 2; ++st)
+            for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = SUM ? 0.f : -delta; }
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    const u32x2 lo = lds_read_tr(kb, t_rd[dt][st][s2][0]);
-                    const u32x2 hv = lds_read_tr(kb, t_rd[dt][st][s2][1]);
-                    dq[dt] = T::mfma32(as_frag<T>(u32x4{lo[0], lo[1], hv[0], hv[1]}), pf[st][s2], dq[dt]);
+            for (int ks = 0; ks < D / 16; ++ks) {
+                s = T::mfma32(as_frag<T>(lds_read128(kb, k_rd[ks] + ro)), qf[ks], s);
+                dp = T::mfma32(as_frag<T>(lds_read128(vb, k_rd[ks] + ro)), df[ks], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], c_log2, -lse2)) * dp[r];
+            // by selection, so that an infinity in a masked place (the lse of a row that sees nothing) adds 0
+            if (masked) {
+                const int j = j0 + 32 * st;
+                const uint32_t m = (seen_bits(j, pos, a.window, a.sinks) & bits_below(klen - j)) >> (4 * hi);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = m & (1u << crow(r, 0)) ? s[r] : 0.f;
+            }
+            if constexpr (SUM) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dsum += s[r];
+                continue;
+            }
+            typename T::frag pf[2];
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                u32x4 pk;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pk[e] = T::pack2(s[8 * s2 + 2 * e], s[8 * s2 + 2 * e + 1]);
+                pf[s2] = as_frag<T>(pk);
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                for (int dt = 0; dt < D / 32; ++dt) {
+                    const int to = ro + 16 * s2 * S::ROW_BYTES;
+                    const u32x2 lo = lds_read_tr(kb, t_rd[dt][0] + to);
+                    const u32x2 hv = lds_read_tr(kb, t_rd[dt][1] + to);
+                    dq[dt] = T::mfma32(as_frag<T>(u32x4{lo[0], lo[1], hv[0], hv[1]}), pf[s2], dq[dt]);
                 }
+        }
     };
-    auto step = [&](auto par, int i) __attribute__((always_inline)) {
+    auto step = [&](auto sum_tag, auto par, int i) __attribute__((always_inline)) {
         constexpr int P = decltype(par)::value;
         if (i + 1 < walk.n) stage(i + 1, 1 - P);
         const int j0 = walk.tile(i) * C::BN;
-        if (rw < R && j0 <= pmax && (j0 + C::BN - 1 > pmin - a.window || j0 < a.sinks)) compute(j0, P);
+        if (rw < R && j0 <= pmax && (j0 + C::BN - 1 > pmin - a.window || j0 < a.sinks)) compute(sum_tag, j0, P);
         vmcnt0();
         __syncthreads();
     };
-    if (walk.n > 0) stage(0, 0);
-    vmcnt0();       // (the compiler's counters see it: the loop inherits no pending prologue load)
-    __syncthreads();
-    for (int i = 0; i < walk.n; i += 2) {
-        step(std::integral_constant<int, 0>(), i);
-        if (i + 1 < walk.n) step(std::integral_constant<int, 1>(), i + 1);
-    }
-
-    if (row >= R) return;
-    uint16_t *op = a.dq + (int64_t)(q_start + t) * a.dq_rs + (int64_t)h * a.dq_hs;
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const int d = 32 * dt + 8 * q4 + 4 * hi;
-            if (d < head_dim)
-                gstore64(op + d, u32x2{T::pack2(dq[dt][4 * q4] * a.scale, dq[dt][4 * q4 + 1] * a.scale),
-                                       T::pack2(dq[dt][4 * q4 + 2] * a.scale, dq[dt][4 * q4 + 3] * a.scale)});
+    auto walk_all = [&](auto sum_tag) __attribute__((always_inline)) {
+        vmcnt0();       // (the compiler's counters see it: the loop inherits no pending prologue load)
+        __syncthreads();
+        for (int i = 0; i < walk.n; i += 2) {
+            step(sum_tag, std::integral_constant<int, 0>(), i);
+            if (i + 1 < walk.n) step(sum_tag, std::integral_constant<int, 1>(), i + 1);
         }
+    };
+    if (walk.n <= WIN_EXACT_TILES) {
+        walk_all(std::true_type{});
+        delta = pair_sum(dsum);
+        if (walk.n > 0) stage(0, 0);
+    }
+    if (hi == 0 && row < R) a.ws_rows[rows_base(a, q_start, sq, kvh) + row] = f32x2{lse2, -delta};
+    walk_all(std::false_type{});
+
+    zero_tail(a.dq, a.dq_rs, a.dq_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
+    store_rows<D, T>(dq, a.scale, smem + wave * 64 * D, head_dim, [&](int r) __attribute__((always_inline)) -> uint16_t * {
+        if (rw + r >= R) return nullptr;
+        const int tt = a.dgroup.div(rw + r), gg = rw + r - tt * G;
+        return a.dq + (int64_t)(q_start + tt) * a.dq_rs + (int64_t)(kvh * G + gg) * a.dq_hs;
+    });
 }
 
 // ------------------------------------------------------------------------------------------- dK, dV
-template <int D, int NW>
+// PAIR: two waves to a block of 32 keys (one computes S, P and dV, the other dP, dS and dK), else one.
+template <int D, int NW, bool PAIR>
 struct WinDkvCfg {
     static constexpr int NT = 64 * NW;
-    static constexpr int BK = 32 * NW;                 // keys per workgroup
+    static constexpr int NB = PAIR ? NW / 2 : NW;      // blocks of 32 keys
+    static constexpr int BK = 32 * NB;                 // keys per workgroup
     static constexpr int BR = 32;                      // packed query rows per step
     static constexpr int NC = D / 8;
     static constexpr int TILE = BR * D * 2;
     static constexpr int PIECES = TILE / 1024;
     static constexpr int PPW = (PIECES + NW - 1) / NW;
     static constexpr int RPP = 1024 / (2 * D);
-    static constexpr int OFF_DO = 2 * TILE;
-    static constexpr int OFF_ROW = 4 * TILE;           // lse[2][BR], delta[2][BR]
-    static constexpr int LDS = OFF_ROW + 4 * BR * 4;
+    static constexpr int STAGE = 2 * TILE + 256;       // Q, dO, row constants
+    static constexpr int RING = PAIR ? 5 : 4;
+    static constexpr int AHEAD = PAIR ? 2 : 3;         // stages in flight
+    static constexpr int DMAS = 2 * PPW + 1;           // a wave's loads per stage
+    static constexpr int OFF_P = RING * STAGE;         // PAIR: P of a step in fp32, two buffers for each pair
+    static constexpr int LDS = OFF_P + (PAIR ? 2 * NB * 4096 : 0);
 };
 
-// A wave owns 32 keys (lane = key), whose K and V rows and dK^T, dV^T stay in registers, and walks the packed
-// query rows that see the workgroup's keys, all heads of the group one after the other: S = Q K^T, dP = dO V^T with
-// Q and dO rows from LDS; P and dS in registers are the B operands of dV^T += dO^T P and dK^T += Q^T dS.
-template <int D, typename T, int NW>
-__global__ __launch_bounds__(64 * NW, D <= 64 ? 2 : 1) void fa_window_dkv_kernel(const WinBwdArgs a) {
-    using C = WinDkvCfg<D, NW>;
+// 64 lanes x 4 bytes to LDS, as dma16
+__device__ __forceinline__ void dma4(i32x4 srd, int voff, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\t"
+                 "buffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(srd), "s"(__builtin_amdgcn_readfirstlane(lds))
+                 : "memory");
+#endif
+}
+
+// A block of 32 keys (lane = key) keeps its K, V rows and dK^T, dV^T in registers and walks the packed query rows that
+// see the workgroup's keys, all heads of the group: S = Q K^T, dP = dO V^T with Q and dO rows from LDS; P and dS in
+// registers are the B operands of dV^T += dO^T P and dK^T += Q^T dS (transposed LDS reads).
+//
+// Tiles of 32 rows come by LDS-DMA into a ring of four stages, three ahead of the compute, so that a step (16 or 32
+// matrix instructions a wave) does not wait for memory; one barrier a step.
+//
+// D = 128 needs 128 registers for dK^T and dV^T alone: there a pair of waves shares the block, each with one of the two
+// accumulators. The P wave leaves P in LDS (fp32: dS takes P unrounded); the dS wave works one step behind it. Each
+// starts a tile's first product a step before it uses it, so a stage is read in three steps, of a ring of five.
+//
+// A sink is seen by every later row, so its block would walk the whole sequence: its rows behind the window are cut
+// into chunks of their own workgroups, in which every block of the workgroup holds the same 32 keys and takes every
+// NB-th tile. Their sums, and the window's for the same keys, go to the workspace and are added in a fixed order
+// by fa_window_sink_sum_kernel.
+template <int D, typename T, int NW, bool PAIR>
+__global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel(const WinBwdArgs a) {
+    using C = WinDkvCfg<D, NW, PAIR>;
     using S = Swz<D>;
     constexpr float LOG2E = 1.4426950408889634f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    float *row_s = (float *)(smem + C::OFF_ROW);
 
-    zero_tail(a.dk, a.dk_rs, a.dk_hs, a.nheads_k, a.head_dim, a.total_k, a.cu_k, a.batch);
-    zero_tail(a.dv, a.dv_rs, a.dv_hs, a.nheads_k, a.head_dim, a.total_k, a.cu_k, a.batch);
-    int w = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int kb = w % a.nblk;
-    w /= a.nblk;
-    const int kvh = w % a.nheads_k;
-    const int b = w / a.nheads_k;
+    auto tails = [&]() __attribute__((always_inline)) {
+        zero_tail(a.dk, a.dk_rs, a.dk_hs, a.nheads_k, a.head_dim, a.total_k, a.cu_k, a.batch);
+        zero_tail(a.dv, a.dv_rs, a.dv_hs, a.nheads_k, a.head_dim, a.total_k, a.cu_k, a.batch);
+    };
+    // the sinks' short workgroups first, then the blocks of keys in an order by XCD
+    const int nsink = a.chunks * a.sink_blocks * a.nheads_k * a.batch;
+    const bool sink = (int)blockIdx.x < nsink;
+    int kb, chunk = 0, w;
+    if (sink) {
+        const int x = a.dchunks.div(blockIdx.x);
+        chunk = blockIdx.x - x * a.chunks;
+        w = a.dsinkb.div(x);
+        kb = x - w * a.sink_blocks;
+    } else {
+        // early keys are seen by the most rows
+        a.order.get(blockIdx.x - nsink, kb, w);
+        kb = a.order.nblk - 1 - kb;
+    }
+    const int b = a.dheads.div(w);
+    const int kvh = w - b * a.nheads_k;
     int q_start, sq, k_start, klen;
     seq_bounds(a.cu_q, b, a.total_q, q_start, sq);
     seq_bounds(a.cu_k, b, a.total_k, k_start, klen);
     const int off = klen - sq;
-    const int G = a.group, k0 = kb * C::BK;
-    if (k0 >= klen) return;
+    const int G = a.group, k0 = kb * (sink ? 32 : C::BK);
+    if (k0 >= klen) {              // (a sink that is not there leaves no sums: its dK, dV have no row)
+        tails();
+        return;
+    }
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hi = lane >> 5;
     const int head_dim = a.head_dim;
-    const int kw = k0 + 32 * wave, key = kw + l32;
+    // block of 32 keys; a pair's waves are NB = 4 apart, on one SIMD: one's matrix work beside the other's exponentials
+    const int blk = wave % C::NB;
+    const bool dswave = PAIR && wave >= C::NB;         // the pair's second wave
+    const int kw = k0 + (sink ? 0 : 32 * blk), key = kw + l32;
 
-    // packed rows that see a key of the block: [r_beg, r_end). Key j is seen from row (j - off) G on, up to row
-    // (j - off + window) G, a sink by every row from there on.
-    const int t_beg = k0 - off > 0 ? k0 - off : 0;
-    int64_t t_end64 = k0 < a.sinks ? sq : (int64_t)k0 + C::BK - 1 + a.window - off;
-    const int t_end = t_end64 < 0 ? 0 : (t_end64 < sq ? (int)t_end64 : sq);
-    const int r_beg = t_beg * G, r_end = t_end * G;
+    // packed rows [r_beg, r_end): key j is seen from row (j - off) G on, up to row (j - off + window) G, a sink by
+    // every row from there on
+    int r_beg, r_end;
+    const bool split = a.chunks > 0;
+    if (sink) {
+        const int64_t t64 = (int64_t)k0 - off + a.window;
+        const int64_t r64 = t64 > 0 ? t64 * G : 0;
+        const int lo = r64 < (int64_t)sq * G ? (int)r64 : sq * G;
+        const int64_t beg = lo + (int64_t)chunk * a.per_chunk;
+        r_beg = beg < (int64_t)sq * G ? (int)beg : sq * G;
+        r_end = r_beg + a.per_chunk < sq * G ? r_beg + a.per_chunk : sq * G;
+    } else {
+        const int t_beg = k0 - off > 0 ? k0 - off : 0;
+        const int64_t t64 = k0 < a.sinks && !split ? sq : (int64_t)k0 + C::BK - 1 + a.window - off;
+        r_beg = t_beg * G;
+        r_end = (t64 < 0 ? 0 : (t64 < sq ? (int)t64 : sq)) * G;
+    }
     const int nt = r_end > r_beg ? (r_end - r_beg + C::BR - 1) / C::BR : 0;
+    // The blocks of a head that run at once see mostly the same rows. Each starts its walk at a tile whose number is a
+    // multiple of the walk's length and goes round, so that they read a tile at the same time, from the L2, instead
+    // of one block's rows a block later, when it has left it.
+    const int rot = sink || nt == 0 ? 0 : (nt - r_beg / C::BR % nt) % nt;
+    auto row_of = [&](int n) __attribute__((always_inline)) -> int {      // first row of the n-th tile walked
+        int u = n + rot;
+        u -= u >= nt ? nt : 0;
+        return r_beg + u * C::BR;
+    };
+    // this lane's rows [lo, up) relative to a tile's first: lane constants, the tile's row is taken off in the loop
+    const int key_lo = (key - off) * G;                                        // first row that sees the key
+    const int64_t key_w = ((int64_t)key - off + a.window) * G;                 // first row behind its window
+    const int key_up = key_w < r_end && !(key < a.sinks && !split) ? (int)key_w : r_end;
+    const int lane_beg = sink ? (key_w > r_end ? r_end : (int)key_w) : key_lo;
+    const int lane_end = sink ? (key < a.sinks ? r_end : lane_beg) : key_up;
 
-    typename T::frag kf[D / 16], vf[D / 16];
+    // ---- staging of tile n: row r is token r / G of head kvh G + r % G; rows behind the last land as zeros
+    const uint16_t *qbase = a.q + (int64_t)q_start * a.q_rs + (int64_t)kvh * G * a.q_hs;
+    const uint16_t *dbase = a.dout + (int64_t)q_start * a.do_rs + (int64_t)kvh * G * a.do_hs;
+    const f32x2 *rows_g = a.ws_rows + rows_base(a, q_start, sq, kvh);
+    int q_off[C::PPW], do_off[C::PPW];                 // from the tile's first token
+    auto lane_offsets = [&](int rt, int t0, int rows) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < C::PPW; ++i) {
+            const int p = (wave + NW * i) % C::PIECES;     // fewer pieces than waves: some are staged twice, alike
+            const int r = C::RPP * p + lane / C::NC, c = (lane % C::NC) ^ S::x(r);
+            const int t = a.dgroup.div(rt + r), g = rt + r - t * G;
+            const bool ok = r < rows && c * 8 < head_dim;
+            q_off[i] = ok ? ((t - t0) * (int)a.q_rs + g * (int)a.q_hs + c * 8) * 2 : OOB;
+            do_off[i] = ok ? ((t - t0) * (int)a.do_rs + g * (int)a.do_hs + c * 8) * 2 : OOB;
+        }
+    };
+    // groups that divide 32 (r_beg and r_end are then whole tokens): a tile's lanes stand alike from its first token,
+    // and rows behind the last are cut off by the descriptor
+    const bool even = 32 % G == 0;
+    if (even) lane_offsets(0, 0, C::BR);
+    int st_buf = 0;                                    // the stage that is filled next
+    auto next_buf = [&](int o) __attribute__((always_inline)) -> int {
+        o += C::STAGE;
+        return o == C::RING * C::STAGE ? 0 : o;
+    };
+    auto stage = [&](int n) __attribute__((always_inline)) {
+        char *buf = smem + st_buf;
+        st_buf = next_buf(st_buf);
+        const int rt = row_of(n);
+        const int t0 = a.dgroup.div(rt);               // the descriptors start at the tile's first token
+        const int left = r_end - rt < C::BR ? r_end - rt : C::BR;
+        int tokens = C::BR + 1;                        // (more than a tile's, within 32 bits: check_rows)
+        if (even)
+            tokens = a.dgroup.div(left);
+        else
+            lane_offsets(rt, t0, left);
+        const i32x4 qs = make_srd(qbase + (int64_t)t0 * a.q_rs, tokens * (int)a.q_rs * 2);
+        const i32x4 ds = make_srd(dbase + (int64_t)t0 * a.do_rs, tokens * (int)a.do_rs * 2);
+#pragma unroll
+        for (int i = 0; i < C::PPW; ++i) {
+            const int p = (wave + NW * i) % C::PIECES;
+            dma16(qs, q_off[i], 0, lds_addr(buf + 1024 * p));
+            dma16(ds, do_off[i], 0, lds_addr(buf + C::TILE + 1024 * p));
+        }
+        // (every wave, the same 256 bytes: a stage is then the same number of loads for each)
+        dma4(make_srd(rows_g + rt, left * 8), lane * 4, lds_addr(buf + 2 * C::TILE));
+    };
+
+    constexpr int AHEAD = C::AHEAD;
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n)
+        if (n < nt) stage(n);
+
+    typename T::frag kf[D / 16], vf[PAIR ? 1 : D / 16];   // PAIR: the wave's own operand, K or V, in kf
     {
         const int kc = key < klen ? key : klen - 1;
         const uint16_t *kp = a.k + (int64_t)(k_start + kc) * a.k_rs + (int64_t)kvh * a.k_hs;
         const uint16_t *vp = a.v + (int64_t)(k_start + kc) * a.v_rs + (int64_t)kvh * a.v_hs;
+        if (dswave) kp = vp;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
             const int c = 2 * ks + hi;
             u32x4 x = {0u, 0u, 0u, 0u}, y = {0u, 0u, 0u, 0u};
             if (c * 8 < head_dim) {
                 x = gload128(kp + c * 8);
-                y = gload128(vp + c * 8);
+                if constexpr (!PAIR) y = gload128(vp + c * 8);
             }
             kf[ks] = as_frag<T>(x);
-            vf[ks] = as_frag<T>(y);
+            if constexpr (!PAIR) vf[ks] = as_frag<T>(y);
         }
     }
-    f32x16 dk[D / 32], dv[D / 32];
+    f32x16 dk[D / 32], dv[PAIR ? 1 : D / 32];             // PAIR: the wave's own accumulator, dV or dK, in dk
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { dk[dt][r] = 0.f; dv[dt][r] = 0.f; }
+        for (int r = 0; r < 16; ++r) {
+            dk[dt][r] = 0.f;
+            if constexpr (!PAIR) dv[dt][r] = 0.f;
+        }
     const float c_log2 = a.scale * LOG2E;
 
-    // ---- staging of one tile of packed rows: row r is token r / G of head kvh G + r % G; rows behind the last
-    // one land as zeros
-    const uint16_t *qbase = a.q + (int64_t)q_start * a.q_rs + (int64_t)kvh * G * a.q_hs;
-    const uint16_t *dbase = a.dout + (int64_t)q_start * a.do_rs + (int64_t)kvh * G * a.do_hs;
-    auto stage = [&](int i, int buf) __attribute__((always_inline)) {
-        const int rt = r_beg + i * C::BR;
-        const int t0 = rt / G;                         // the descriptor starts at the tile's first token
-        const i32x4 qs = make_srd(qbase + (int64_t)t0 * a.q_rs, 0x7FFFFFFF);
-        const i32x4 ds = make_srd(dbase + (int64_t)t0 * a.do_rs, 0x7FFFFFFF);
-#pragma unroll
-        for (int n = 0; n < C::PPW; ++n) {
-            const int p = wave + NW * n;
-            if (C::PIECES % NW == 0 || p < C::PIECES) {
-                const int r = C::RPP * p + lane / C::NC;
-                const int c = (lane % C::NC) ^ S::x(r);
-                const int t = (rt + r) / G, g = rt + r - t * G;
-                const bool ok = rt + r < r_end && c * 8 < head_dim;
-                const int qo = ok ? ((t - t0) * (int)a.q_rs + g * (int)a.q_hs + c * 8) * 2 : OOB;
-                const int dof = ok ? ((t - t0) * (int)a.do_rs + g * (int)a.do_hs + c * 8) * 2 : OOB;
-                dma16(qs, qo, 0, lds_addr(smem + buf * C::TILE + 1024 * p));
-                dma16(ds, dof, 0, lds_addr(smem + C::OFF_DO + buf * C::TILE + 1024 * p));
-            }
-        }
-    };
-    // lse and delta of the tile's rows: loaded by the first 32 lanes a step ahead, written at the step's end
-    float lse_st = 0.f, del_st = 0.f;
-    auto load_rows = [&](int i) __attribute__((always_inline)) {
-        if (tid < C::BR) {
-            int r = r_beg + i * C::BR + tid;
-            r = r < r_end ? r : r_end - 1;
-            const int t = r / G, g = r - t * G;
-            const int64_t li = (int64_t)(b * a.nheads + kvh * G + g) * a.lse_stride + t;
-            lse_st = a.lse[li] * LOG2E;
-            del_st = -a.delta[li];
-        }
-    };
-    auto store_rows = [&](int buf) __attribute__((always_inline)) {
-        if (tid < C::BR) {
-            row_s[buf * C::BR + tid] = lse_st;
-            row_s[(2 + buf) * C::BR + tid] = del_st;
-        }
-    };
-
     const int grp = (lane >> 4) & 1, qq = (lane & 15) >> 2, pp = lane & 3;
-    auto compute = [&](int i, int buf) __attribute__((always_inline)) {
-        const char *qb = smem + buf * C::TILE, *db = smem + C::OFF_DO + buf * C::TILE;
-        const float *lse_b = row_s + buf * C::BR, *del_b = row_s + (2 + buf) * C::BR;
-        const int rt = r_beg + i * C::BR;
-        f32x16 s, dp;
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            const f32x4 d4 = *reinterpret_cast<const f32x4 *>(del_b + 8 * q4 + 4 * hi);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { s[4 * q4 + e] = 0.f; dp[4 * q4 + e] = d4[e]; }   // dP starts at -delta
-        }
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const int ro = S::off(l32, 2 * ks + hi);
-            s = T::mfma32(as_frag<T>(lds_read128(qb, ro)), kf[ks], s);
-            dp = T::mfma32(as_frag<T>(lds_read128(db, ro)), vf[ks], dp);
-        }
-        // rows of the tile that see this lane's key, as bits
-        const int lo = (key - off) * G - rt;
-        const int64_t up64 = key < a.sinks ? (int64_t)r_end - rt : (int64_t)(key - off + (int64_t)a.window) * G - rt;
-        const int up = (int)(up64 < 0 ? 0 : (up64 > 32 ? 32 : up64));
-        uint32_t m = bits_below(up) & ~bits_below(lo) & bits_below(r_end - rt);
-        if (key >= klen) m = 0;
-        const bool whole = __builtin_amdgcn_ballot_w64(m != 0xFFFFFFFFu) == 0;
-        m >>= 4 * hi;
-        auto pds = [&](auto masked_tag) __attribute__((always_inline)) {
-            constexpr bool MASKED = decltype(masked_tag)::value;
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(lse_b + 8 * q4 + 4 * hi);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * q4 + e;
-                    const bool dead = MASKED && !(m & (1u << crow(r, 0)));
-                    const float p = fast_exp2(fmaf(s[r], c_log2, -l4[e]));
-                    const float x = p * dp[r];
-                    s[r] = dead ? 0.f : p;
-                    dp[r] = dead ? 0.f : x;
-                }
-            }
-        };
-        if (whole)
-            pds(std::false_type{});
-        else
-            pds(std::true_type{});
-        u32x4 pk[2], sk[2];
-#pragma unroll
-        for (int sg = 0; sg < 2; ++sg)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                pk[sg][e] = T::pack2(s[8 * sg + 2 * e], s[8 * sg + 2 * e + 1]);
-                sk[sg][e] = T::pack2(dp[8 * sg + 2 * e], dp[8 * sg + 2 * e + 1]);
-            }
+    // The swizzles exclusive-or a chunk's number with bits of its row: k-step ks of a row read is the lane's address ^
+    // 32 ks, column block dt of a transposed read ^ 64 dt, eight rows further on ^ 32 (images start at whole rows). One
+    // register each instead of one for each read.
+    static_assert(C::STAGE % S::ROW_BYTES == 0 && C::TILE % S::ROW_BYTES == 0, "images at whole rows");
+    const int r_rd = S::off(l32, hi), t_rd = S::off8(4 * hi + qq, 16 * grp + 4 * pp);
+    // X^T += A^T B over the tile's 32 rows: A rows in LDS (transposed reads), B packed in registers
+    auto add_t = [&](f32x16 (&x)[D / 32], int rows, const u32x4 (&bv)[2]) __attribute__((always_inline)) {
+        const int at = rows + t_rd;
 #pragma unroll
         for (int sg = 0; sg < 2; ++sg)
 #pragma unroll
             for (int dt = 0; dt < D / 32; ++dt) {
-                const int r = 16 * sg + 4 * hi + qq, col = 32 * dt + 16 * grp + 4 * pp;
-                const int o0 = S::off8(r, col), o1 = S::off8(r + 8, col);
-                const u32x2 a0 = lds_read_tr(db, o0), a1 = lds_read_tr(db, o1);
-                dv[dt] = T::mfma32(as_frag<T>(u32x4{a0[0], a0[1], a1[0], a1[1]}), as_frag<T>(pk[sg]), dv[dt]);
-                const u32x2 b0 = lds_read_tr(qb, o0), b1 = lds_read_tr(qb, o1);
-                dk[dt] = T::mfma32(as_frag<T>(u32x4{b0[0], b0[1], b1[0], b1[1]}), as_frag<T>(sk[sg]), dk[dt]);
+                const int ro = 16 * sg * S::ROW_BYTES;
+                const u32x2 a0 = lds_read_tr(smem, (at ^ (dt << 6)) + ro);
+                const u32x2 a1 = lds_read_tr(smem, (at ^ (dt << 6) ^ 32) + ro + 8 * S::ROW_BYTES);
+                x[dt] = T::mfma32(as_frag<T>(u32x4{a0[0], a0[1], a1[0], a1[1]}), as_frag<T>(bv[sg]), x[dt]);
             }
     };
-    // a wave skips a tile that sees none of its 32 keys
-    const int w_lo = (kw - off) * G;
-    const int64_t w_up = kw < a.sinks ? (int64_t)r_end : (int64_t)((int64_t)kw + 31 - off + a.window) * G;
-    auto step = [&](auto par, int i) __attribute__((always_inline)) {
-        constexpr int P = decltype(par)::value;
-        if (i + 1 < nt) {
-            stage(i + 1, 1 - P);
-            load_rows(i + 1);
-        }
-        const int rt = r_beg + i * C::BR;
-        if (kw < klen && rt + C::BR > w_lo && rt < w_up) compute(i, P);
-        if (i + 1 < nt) store_rows(1 - P);
-        vmcnt0();
-        __syncthreads();
-    };
-    if (nt > 0) {
-        stage(0, 0);
-        load_rows(0);
-        store_rows(0);
-    }
-    vmcnt0();
-    __syncthreads();
-    for (int i = 0; i < nt; i += 2) {
-        step(std::integral_constant<int, 0>(), i);
-        if (i + 1 < nt) step(std::integral_constant<int, 1>(), i + 1);
-    }
-
-    if (key >= klen) return;
-    uint16_t *kp = a.dk + (int64_t)(k_start + key) * a.dk_rs + (int64_t)kvh * a.dk_hs;
-    uint16_t *vp = a.dv + (int64_t)(k_start + key) * a.dv_rs + (int64_t)kvh * a.dv_hs;
+    auto pack = [&](const f32x16 &x, u32x4 (&out)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+        for (int sg = 0; sg < 2; ++sg)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out[sg][e] = T::pack2(x[8 * sg + 2 * e], x[8 * sg + 2 * e + 1]);
+    };
+    // the tile's rows as A operands, all on their way before the first is used
+    auto read_rows = [&](int rows, u32x4 (&x)[D / 16]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) x[ks] = lds_read128(smem, (rows + r_rd) ^ (ks << 5));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // P of tile n: 0 (by selection: an infinity may stand there) in the rows that do not see this lane's key. Most
+    // tiles are seen whole; the empty asm keeps the branch a branch.
+    auto mask_p = [&](int n, f32x16 &p) __attribute__((always_inline)) {
+        const int rt = row_of(n);
+        uint32_t m = bits_below(lane_end - rt) & ~bits_below(lane_beg - rt);
+        if (key >= klen) m = 0;
+        if (__builtin_amdgcn_ballot_w64(m != 0xFFFFFFFFu) == 0) return;
+        asm volatile("");
+        m >>= 4 * hi;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = m & (1u << crow(r, 0)) ? p[r] : 0.f;
+    };
+    // does the block take tile n?
+    const int w_lo = (kw - off) * G;
+    const int64_t w_up = kw < a.sinks && !split ? (int64_t)r_end : ((int64_t)kw + 31 - off + a.window) * G;
+    auto takes = [&](int n) __attribute__((always_inline)) -> bool {
+        const int rt = row_of(n);
+        return sink ? n % C::NB == blk : (kw < klen && rt + C::BR > w_lo && rt < w_up);
+    };
+    // row constants of registers 4 q4 .. 4 q4 + 3 (rows 8 q4 + 4 hi + e): {lse2, -delta} pairs
+    auto row_consts = [&](int buf, int q4, float (&l)[4], float (&d)[4]) __attribute__((always_inline)) {
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(smem + buf + 2 * C::TILE + (8 * q4 + 4 * hi) * 8);
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(smem + buf + 2 * C::TILE + (8 * q4 + 4 * hi) * 8 + 16);
+        l[0] = x[0]; d[0] = x[1]; l[1] = x[2]; d[1] = x[3];
+        l[2] = y[0]; d[2] = y[1]; l[3] = y[2]; d[3] = y[3];
+    };
+    auto compute_one = [&](int n, int buf) __attribute__((always_inline)) {
+        f32x16 s, dp;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            const int d = 32 * dt + 8 * q4 + 4 * hi;
-            if (d < head_dim) {
-                gstore64(kp + d, u32x2{T::pack2(dk[dt][4 * q4] * a.scale, dk[dt][4 * q4 + 1] * a.scale),
-                                       T::pack2(dk[dt][4 * q4 + 2] * a.scale, dk[dt][4 * q4 + 3] * a.scale)});
-                gstore64(vp + d, u32x2{T::pack2(dv[dt][4 * q4], dv[dt][4 * q4 + 1]),
-                                       T::pack2(dv[dt][4 * q4 + 2], dv[dt][4 * q4 + 3])});
+            float l[4], d[4];
+            row_consts(buf, q4, l, d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[4 * q4 + e] = 0.f;
+                dp[4 * q4 + e] = d[e];                 // dP starts at -delta
             }
         }
+        // (operands read two k-steps at a time: all at once, as in a pair, took 81 us for 72 here, the registers short)
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            s = T::mfma32(as_frag<T>(lds_read128(smem, (buf + r_rd) ^ (ks << 5))), kf[ks], s);
+            dp = T::mfma32(as_frag<T>(lds_read128(smem, (buf + C::TILE + r_rd) ^ (ks << 5))), vf[PAIR ? 0 : ks], dp);
+            if (ks % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            float l[4], d[4];
+            row_consts(buf, q4, l, d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fast_exp2(fmaf(s[4 * q4 + e], c_log2, -l[e]));
+        }
+        mask_p(n, s);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+        u32x4 pk[2], sk[2];
+        pack(s, pk);
+        pack(dp, sk);
+        if constexpr (!PAIR) {
+            add_t(dv, buf + C::TILE, pk);
+            add_t(dk, buf, sk);
+        }
+    };
+    // PAIR: S of a tile (P wave) or dP (dS wave), started one step before the rest of its work, so that the matrix
+    // instructions of one tile run under the exponentials, LDS traffic and packing of the one before
+    auto first_p = [&](int buf, f32x16 &s) __attribute__((always_inline)) {
+        u32x4 x[D / 16];
+        read_rows(buf, x);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) s = T::mfma32(as_frag<T>(x[ks]), kf[ks], s);
+    };
+    auto rest_p = [&](int n, int buf, f32x16 s) __attribute__((always_inline)) {
+        char *img = smem + C::OFF_P + (2 * blk + (n & 1)) * 4096;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            float l[4], d[4];
+            row_consts(buf, q4, l, d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fast_exp2(fmaf(s[4 * q4 + e], c_log2, -l[e]));
+        }
+        mask_p(n, s);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<f32x4 *>(img + (q4 * 64 + lane) * 16) = f32x4{s[4 * q4], s[4 * q4 + 1], s[4 * q4 + 2], s[4 * q4 + 3]};
+        u32x4 pk[2];
+        pack(s, pk);
+        add_t(dk, buf + C::TILE, pk);                  // dV^T
+    };
+    auto first_ds = [&](int buf, f32x16 &dp) __attribute__((always_inline)) {
+        u32x4 y[D / 16];
+        read_rows(buf + C::TILE, y);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            float l[4], d[4];
+            row_consts(buf, q4, l, d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = d[e];
+        }
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) dp = T::mfma32(as_frag<T>(y[ks]), kf[ks], dp);
+    };
+    auto rest_ds = [&](int n, int buf, f32x16 dp) __attribute__((always_inline)) {
+        const char *img = smem + C::OFF_P + (2 * blk + (n & 1)) * 4096;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+            const f32x4 p = *reinterpret_cast<const f32x4 *>(img + (q4 * 64 + lane) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * q4 + e] *= p[e];
+        }
+        u32x4 sk[2];
+        pack(dp, sk);
+        add_t(dk, buf, sk);                            // dK^T
+    };
+
+    // ---- the walk
+    vmcnt0();
+    auto arrive = [&](int n) __attribute__((always_inline)) {
+        // tile n has landed when at most the later stages' loads are out
+        if (n + AHEAD - 1 < nt)
+            vmcnt_n<C::DMAS *(AHEAD - 1)>();
+        else if (AHEAD == 3 && n + 1 < nt)
+            vmcnt_n<C::DMAS>();
+        else
+            vmcnt0();
+        __syncthreads();
+        if (n + AHEAD < nt) stage(n + AHEAD);
+    };
+    if constexpr (!PAIR) {
+        int buf = 0;
+        for (int n = 0; n < nt; ++n) {
+            arrive(n);
+            if (takes(n)) compute_one(n, buf);
+            buf = next_buf(buf);
+        }
+    } else {
+        // Step k of nt + 2: the P wave starts tile k and ends tile k - 1, the dS wave starts k - 1 and ends k - 2, whose
+        // P the other left a step before. A loop for each (one loop with a branch moved the accumulators), with the
+        // same barriers.
+        auto walk = [&](auto lag_tag, auto &&first, auto &&rest) __attribute__((always_inline)) {
+            constexpr int LAG = decltype(lag_tag)::value;
+            f32x16 cur, next;
+            for (int k = 0; k <= LAG; ++k) arrive(k);
+            if (!sink) {
+                // a tile that a block does not see goes through with P = 0: the barriers set the pace, and without
+                // a branch the accumulators stay where they are
+                first(0, cur);
+                int buf = 0;
+                for (int n = 1; n < nt; ++n) {
+                    arrive(n + LAG);
+                    const int at = next_buf(buf);
+                    first(at, next);
+                    rest(n - 1, buf, cur);
+                    cur = next;
+                    buf = at;
+                }
+                arrive(nt + LAG);
+                rest(nt - 1, buf, cur);
+            } else {
+                int buf = 0;
+                for (int n = 0; n < nt; ++n) {
+                    if (takes(n)) first(buf, cur);
+                    arrive(n + 1 + LAG);
+                    if (takes(n)) rest(n, buf, cur);
+                    buf = next_buf(buf);
+                }
+            }
+            for (int k = nt + 1 + LAG; k < nt + 2; ++k) arrive(k);
+        };
+        if (nt > 0) {
+            if (!dswave)
+                walk(std::integral_constant<int, 0>(), first_p, rest_p);
+            else
+                walk(std::integral_constant<int, 1>(), first_ds, rest_ds);
+        }
+    }
+
+    tails();
+    __syncthreads();       // the ring is free: rows go out through it
+    auto store = [&](const f32x16 (&x)[D / 32], bool is_v) __attribute__((always_inline)) {
+        if (split && key < a.sinks && key < klen) {
+            const int slot = sink ? chunk * C::NB + blk : a.slots - 1;
+            float *pp_ = a.ws_part + ((((int64_t)(b * a.nheads_k + kvh) * a.sinks + key) * a.slots + slot) * 2 + (is_v ? 1 : 0)) * D;
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4)
+                    *reinterpret_cast<f32x4 *>(pp_ + 32 * dt + 8 * q4 + 4 * hi) = f32x4{x[dt][4 * q4], x[dt][4 * q4 + 1], x[dt][4 * q4 + 2], x[dt][4 * q4 + 3]};
+        }
+        if (sink) return;
+        const int64_t rs = is_v ? a.dv_rs : a.dk_rs, hs = is_v ? a.dv_hs : a.dk_hs;
+        uint16_t *base = (is_v ? a.dv : a.dk) + (int64_t)(k_start + kw) * rs + (int64_t)kvh * hs;
+        store_rows<D, T>(x, is_v ? 1.f : a.scale, smem + wave * 64 * D, head_dim, [&](int r) __attribute__((always_inline)) -> uint16_t * {
+            return kw + r >= klen || (split && kw + r < a.sinks) ? nullptr : base + r * rs;
+        });
+    };
+    if constexpr (PAIR) {
+        store(dk, !dswave);
+    } else {
+        store(dv, true);
+        store(dk, false);
+    }
+}
+
+// The sinks' dK and dV: their parts in the parts' order, rounded once. A workgroup to a key and head; its quarters
+// take a quarter of the parts each, eight loads in flight.
+template <int D, typename T>
+__global__ __launch_bounds__(8 * D) void fa_window_sink_sum_kernel(const WinBwdArgs a) {
+    __shared__ float quarter[4][2 * D];
+    const int key = blockIdx.x, bh = blockIdx.y, b = a.dheads.div(bh), kvh = bh - b * a.nheads_k;
+    int k_start, klen;
+    seq_bounds(a.cu_k, b, a.total_k, k_start, klen);
+    if (key >= klen) return;
+    const int x = threadIdx.x % (2 * D), part = threadIdx.x / (2 * D), is_v = x / D, d = x % D;
+    const int per = (a.slots + 3) / 4, beg = part * per, end = beg + per < a.slots ? beg + per : a.slots;
+    const float *p = a.ws_part + ((int64_t)bh * a.sinks + key) * a.slots * 2 * D + x;
+    float sum = 0.f;
+    for (int s = beg; s < end; s += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = s + i < end ? p[(int64_t)(s + i) * 2 * D] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += v[i];
+    }
+    quarter[part][x] = sum;
+    __syncthreads();
+    if (part > 0 || d >= a.head_dim) return;
+    sum = (quarter[0][x] + quarter[1][x]) + (quarter[2][x] + quarter[3][x]);
+    if (is_v)
+        a.dv[(int64_t)(k_start + key) * a.dv_rs + (int64_t)kvh * a.dv_hs + d] = T::from_float(sum);
+    else
+        a.dk[(int64_t)(k_start + key) * a.dk_rs + (int64_t)kvh * a.dk_hs + d] = T::from_float(sum * a.scale);
 }
 
 }  // namespace fa

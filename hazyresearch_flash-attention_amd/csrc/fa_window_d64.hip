@@ -3,5 +3,5 @@
 
 namespace fa {
 template hipError_t launch_window_fwd<64>(const WinFwdArgs &, int, bool, WinShape, hipStream_t);
-template hipError_t launch_window_bwd<64>(const WinBwdArgs &, int, int, int, hipStream_t);
+template hipError_t launch_window_bwd<64>(const WinBwdArgs &, int, const WinBwdPlan &, hipStream_t);
 }  // namespace fa

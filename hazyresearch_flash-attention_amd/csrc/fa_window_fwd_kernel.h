@@ -33,6 +33,8 @@ struct WinFwdArgs {
     int num_pages, page_shift, num_seqs, max_blocks, tree_words;
     int lse_stride, window, sinks, nrb, nsplit;
     float scale;
+    Div dgroup, dheads, dsplit;   // by group, nheads_k, nsplit
+    BlockOrder order;             // dense; paged: its blk divides by nrb
 };
 
 __device__ __forceinline__ float wmax3(float a, float b, float c) {
@@ -69,17 +71,20 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     constexpr float LN2 = 0.6931471805599453f;
     extern __shared__ __attribute__((aligned(16))) char smem[];
 
-    zero_tail(a.o, a.o_rs, a.o_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
-    // ---- block -> (row block, split, key/value head, sequence). The row blocks of one split share its K/V, and
-    // a head's blocks follow each other, so that an XCD's L2 holds what its workgroups read; late row blocks
-    // (which see more keys while the window fills) come first.
-    int w = xcd_contiguous(blockIdx.x, gridDim.x);
-    const int rb = a.nrb - 1 - w % a.nrb;
-    w /= a.nrb;
-    const int split = w % a.nsplit;
-    w /= a.nsplit;
-    const int kvh = w % a.nheads_k;
-    const int b = w / a.nheads_k;
+    // ---- block -> (row block, split, key/value head, sequence). The row blocks of one split of a paged call share
+    // its K/V and follow each other.
+    int rb, split = 0, w;
+    if constexpr (PAGED) {
+        w = xcd_contiguous(blockIdx.x, gridDim.x);
+        int x = a.order.blk.div(w);
+        rb = w - x * a.nrb;
+        w = a.dsplit.div(x);
+        split = x - w * a.nsplit;
+    } else {
+        a.order.get(blockIdx.x, rb, w);
+    }
+    const int b = a.dheads.div(w);
+    const int kvh = w - b * a.nheads_k;
 
     int q_start, sq, klen, off;
     const uint16_t *kbase, *vbase;
@@ -89,7 +94,10 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     const int G = a.group;
     const int R = sq * G;
     const int r0 = rb * C::BM;
-    if (r0 >= R) return;
+    if (r0 >= R) {
+        zero_tail(a.o, a.o_rs, a.o_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
+        return;
+    }
     if constexpr (PAGED) {
         const int row = a.seq_ids ? a.seq_ids[b] : b;
         const bool used = row >= 0 && row < a.num_seqs;
@@ -122,12 +130,13 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     const int rw = r0 + 32 * wr;                              // first row of the wave
     const int row = rw + l32;
     const int rc = row < R ? row : R - 1;                     // rows behind the end compute what nobody stores
-    const int t = rc / G, g = rc - t * G;
+    const int t = a.dgroup.div(rc), g = rc - t * G;
     int pos = off + t;
-    int pmin = off + rw / G, pmax = off + (rw + 31 < R ? rw + 31 : R - 1) / G;   // positions of the wave
+    // positions of the wave
+    int pmin = off + a.dgroup.div(rw), pmax = off + a.dgroup.div(rw + 31 < R ? rw + 31 : R - 1);
     if (rw >= R) pmin = pmax = pos;
-    int bmin = off + r0 / G;                                  // of the workgroup
-    int k_end = off + (r0 + C::BM < R ? r0 + C::BM - 1 : R - 1) / G + 1;
+    int bmin = off + a.dgroup.div(r0);                        // of the workgroup
+    int k_end = off + a.dgroup.div(r0 + C::BM < R ? r0 + C::BM - 1 : R - 1) + 1;
     int *depth_s = (int *)(smem + C::TREE_OFF);
     const uint64_t *my_mask = nullptr;
     if constexpr (TREE) {
@@ -146,30 +155,10 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     }
     k_end = k_end < klen ? k_end : klen;
     const TileWalk walk = tile_walk(bmin, k_end, a.window, a.sinks, BN);
-    const int per = (walk.n + a.nsplit - 1) / a.nsplit;
+    const int per = a.dsplit.div(walk.n + a.nsplit - 1);
     const int i_beg = split * per;
     const int i_end = walk.n < i_beg + per ? walk.n : i_beg + per;
     const int steps = i_end > i_beg ? (i_end - i_beg + KG - 1) / KG : 0;
-
-    // ---- Q: B operand of S^T = K Q^T, element j of k-step ks is Q[row][16 ks + 8 hi + j]. A negative scale
-    // turns Q's sign, a zero scale makes it 0, so that the running maximum is always of c * s with c > 0.
-    const float c_log2 = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * LOG2E;
-    typename T::frag qf[D / 16];
-    {
-        const uint16_t *qp = a.q + (int64_t)(q_start + t) * a.q_rs + (int64_t)(kvh * G + g) * a.q_hs;
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            const int c = 2 * ks + hi;
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (c * 8 < head_dim && a.scale != 0.f) {
-                x = gload128(qp + c * 8);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] ^= flip;
-            }
-            qf[ks] = as_frag<T>(x);
-        }
-    }
 
     // ---- staging. Piece p (1 KiB = RPP rows) is written by row wave p % NWR of its group; lane l lands at byte
     // 16 l of the piece, so the swizzle goes onto the source: slot l % NC of row RPP p + l / NC holds chunk
@@ -241,6 +230,35 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         }
         return there;
     };
+
+    // ---- the first tile is on its way before the rows are read
+    auto idx = [&](int n) __attribute__((always_inline)) -> int { return i_beg + KG * n + kg; };
+    uint32_t there = 0, there_n = 0;
+    if (idx(0) < i_end) {
+        load_entries(idx(0));
+        there = stage(idx(0), 0);
+    }
+    if (idx(1) < i_end) load_entries(idx(1));
+
+    // ---- Q: B operand of S^T = K Q^T, element j of k-step ks is Q[row][16 ks + 8 hi + j]. A negative scale
+    // turns Q's sign, a zero scale makes it 0, so that the running maximum is always of c * s with c > 0.
+    const float c_log2 = (a.scale == 0.f ? 1.f : fabsf(a.scale)) * LOG2E;
+    typename T::frag qf[D / 16];
+    {
+        const uint16_t *qp = a.q + (int64_t)(q_start + t) * a.q_rs + (int64_t)(kvh * G + g) * a.q_hs;
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            const int c = 2 * ks + hi;
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (c * 8 < head_dim && a.scale != 0.f) {
+                x = gload128(qp + c * 8);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] ^= flip;
+            }
+            qf[ks] = as_frag<T>(x);
+        }
+    }
 
     // ---- lane-constant LDS offsets: K rows, and V^T by transposed reads
     const int grp = (lane >> 4) & 1, qq = (lane & 15) >> 2, pp = lane & 3;
@@ -381,7 +399,6 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     };
 
     // ---- the walk: stage tile n+1, compute tile n, wait, meet
-    auto idx = [&](int n) __attribute__((always_inline)) -> int { return i_beg + KG * n + kg; };
     auto meet = [&]() __attribute__((always_inline)) {
         vmcnt0();
         if constexpr (NWR > 1) {
@@ -392,15 +409,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
             asm volatile("" ::: "memory");
         }
     };
-    uint32_t there = 0, there_n = 0;
-    if (steps > 0) {
-        if (idx(0) < i_end) {
-            load_entries(idx(0));
-            there = stage(idx(0), 0);
-        }
-        if (idx(1) < i_end) load_entries(idx(1));
-        meet();
-    }
+    if (steps > 0) meet();
     auto step = [&](auto par, int n) __attribute__((always_inline)) {
         constexpr int P = decltype(par)::value;
         const int i = idx(n);
@@ -419,6 +428,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         if (n + 1 < steps) step(std::integral_constant<int, 1>(), n + 1);
     }
 
+    zero_tail(a.o, a.o_rs, a.o_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
     float l_tot = pair_sum(l_i);
     float mrow = m_thr == -INFINITY ? -INFINITY : mc;         // m * c_log2, -inf: nothing seen
 
@@ -467,8 +477,9 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         }
         mrow = top;
     }
-    if (row >= R) return;
-
+    if (KG > 1 || a.nsplit > 1) {
+        if (row >= R) return;
+    }
     if (a.nsplit > 1) {
         const int64_t wrow = ((int64_t)split * a.total_q + q_start + t) * a.nheads + kvh * G + g;
         float *op = a.ws_o + wrow * D;
@@ -485,24 +496,33 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         return;
     }
 
-    // ---- epilogue: O / l in 16 bits; lanes l and l + 32 hold the halves of each group of 8 columns, one lane
-    // exchange gives each a whole 16-byte store
+    // ---- epilogue: O / l in 16 bits
     const bool empty = mrow == -INFINITY && l_tot == 0.f;
     const float inv = empty ? 0.f : 1.f / l_tot;
-    uint16_t *op = a.o + (int64_t)(q_start + t) * a.o_rs + (int64_t)(kvh * G + g) * a.o_hs;
+    if constexpr (KG == 1) {
+        store_rows<D, T>(o, inv, smem + wave * 64 * D, head_dim, [&](int r) __attribute__((always_inline)) -> uint16_t * {
+            if (rw + r >= R) return nullptr;
+            const int tt = a.dgroup.div(rw + r), gg = rw + r - tt * G;
+            return a.o + (int64_t)(q_start + tt) * a.o_rs + (int64_t)(kvh * G + gg) * a.o_hs;
+        });
+        if (row >= R) return;
+    } else {
+        // lanes l and l + 32 hold the halves of each group of 8 columns; one exchange gives each a 16-byte store
+        uint16_t *op = a.o + (int64_t)(q_start + t) * a.o_rs + (int64_t)(kvh * G + g) * a.o_hs;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+        for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int g4 = 0; g4 < 4; g4 += 2) {
-            const uint32_t a0 = T::pack2(o[dt][4 * g4 + 0] * inv, o[dt][4 * g4 + 1] * inv);
-            const uint32_t a1 = T::pack2(o[dt][4 * g4 + 2] * inv, o[dt][4 * g4 + 3] * inv);
-            const uint32_t b0 = T::pack2(o[dt][4 * g4 + 4] * inv, o[dt][4 * g4 + 5] * inv);
-            const uint32_t b1 = T::pack2(o[dt][4 * g4 + 6] * inv, o[dt][4 * g4 + 7] * inv);
-            const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
-            const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
-            const int d = 32 * dt + 8 * (g4 + hi);
-            if (d < head_dim) gstore128(op + d, u32x4{s0[0], s1[0], s0[1], s1[1]});
-        }
+            for (int g4 = 0; g4 < 4; g4 += 2) {
+                const uint32_t a0 = T::pack2(o[dt][4 * g4 + 0] * inv, o[dt][4 * g4 + 1] * inv);
+                const uint32_t a1 = T::pack2(o[dt][4 * g4 + 2] * inv, o[dt][4 * g4 + 3] * inv);
+                const uint32_t b0 = T::pack2(o[dt][4 * g4 + 4] * inv, o[dt][4 * g4 + 5] * inv);
+                const uint32_t b1 = T::pack2(o[dt][4 * g4 + 6] * inv, o[dt][4 * g4 + 7] * inv);
+                const auto s0 = __builtin_amdgcn_permlane32_swap(a0, b0, false, false);
+                const auto s1 = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+                const int d = 32 * dt + 8 * (g4 + hi);
+                if (d < head_dim) gstore128(op + d, u32x4{s0[0], s1[0], s0[1], s1[1]});
+            }
+    }
     if (hi == 0 && a.lse)
         a.lse[(int64_t)(b * a.nheads + kvh * G + g) * a.lse_stride + t] = empty ? -INFINITY : mrow * LN2 + __logf(l_tot);
 }

@@ -19,7 +19,7 @@ static hipError_t launch_window_fwd_k(const WinFwdArgs &a, hipStream_t s) {
 
 template <int D, typename T>
 static hipError_t launch_window_fwd_t(const WinFwdArgs &a, bool paged, WinShape shape, hipStream_t s) {
-    if (!paged) return launch_window_fwd_k<D, T, 4, 1, 64, false, false>(a, s);
+    if (!paged) return launch_window_fwd_k<D, T, WIN_FWD_WAVES, 1, WIN_FWD_KEYS, false, false>(a, s);
     hipError_t e;
     const bool tree = a.tree != nullptr;
     switch (shape) {
@@ -50,32 +50,36 @@ hipError_t launch_window_fwd(const WinFwdArgs &a, int dtype, bool paged, WinShap
 }
 
 template <int D, typename T>
-static hipError_t launch_window_bwd_t(WinBwdArgs a, int max_rows, int max_k, hipStream_t s) {
-    constexpr int NW = 4;
-    if (max_rows > 0) {
-        using C = WinDqCfg<D, NW>;
-        auto kern = fa_window_dq_kernel<D, T, NW>;
+static hipError_t launch_window_bwd_t(WinBwdArgs a, const WinBwdPlan &p, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    if (p.max_rows > 0) {
+        using C = WinDqCfg<D, WIN_DQ_WAVES>;
+        auto kern = fa_window_dq_kernel<D, T, WIN_DQ_WAVES>;
         FA_ENSURE_LDS(kern, C::LDS);
-        a.nblk = (max_rows + C::BM - 1) / C::BM;
-        hipLaunchKernelGGL(kern, dim3((uint32_t)((int64_t)a.nblk * a.nheads_k * a.batch)), dim3(C::NT), C::LDS, s, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        a.order = BlockOrder::of((p.max_rows + C::BM - 1) / C::BM, a.nheads_k * a.batch, p.order);
+        hipLaunchKernelGGL(kern, dim3((uint32_t)((int64_t)a.order.nblk * a.order.nbh)), dim3(C::NT), C::LDS, s, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    if (max_k > 0) {
-        using C = WinDkvCfg<D, NW>;
-        auto kern = fa_window_dkv_kernel<D, T, NW>;
+    if (p.max_k > 0) {
+        using C = WinDkvCfg<D, win_dkv_waves(D), D == 128>;
+        auto kern = fa_window_dkv_kernel<D, T, win_dkv_waves(D), D == 128>;
         FA_ENSURE_LDS(kern, C::LDS);
-        a.nblk = (max_k + C::BK - 1) / C::BK;
-        hipLaunchKernelGGL(kern, dim3((uint32_t)((int64_t)a.nblk * a.nheads_k * a.batch)), dim3(C::NT), C::LDS, s, a);
-        return hipGetLastError();
+        static_assert(C::NB == WIN_DKV_BLOCKS, "the plan's blocks");
+        a.order = BlockOrder::of((p.max_k + C::BK - 1) / C::BK, a.nheads_k * a.batch, p.order);
+        const int64_t wgs = ((int64_t)a.order.nblk + (int64_t)a.chunks * a.sink_blocks) * a.order.nbh;
+        hipLaunchKernelGGL(kern, dim3((uint32_t)wgs), dim3(C::NT), C::LDS, s, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        if (a.chunks > 0) {
+            hipLaunchKernelGGL((fa_window_sink_sum_kernel<D, T>), dim3(a.sinks, a.nheads_k * a.batch), dim3(8 * D), 0, s, a);
+            e = hipGetLastError();
+        }
     }
-    return hipSuccess;
+    return e;
 }
 
 template <int D>
-hipError_t launch_window_bwd(const WinBwdArgs &a, int dtype, int max_rows, int max_k, hipStream_t s) {
-    return dtype == FA_DTYPE_BF16 ? launch_window_bwd_t<D, Bf16>(a, max_rows, max_k, s)
-                                  : launch_window_bwd_t<D, Fp16>(a, max_rows, max_k, s);
+hipError_t launch_window_bwd(const WinBwdArgs &a, int dtype, const WinBwdPlan &p, hipStream_t s) {
+    return dtype == FA_DTYPE_BF16 ? launch_window_bwd_t<D, Bf16>(a, p, s) : launch_window_bwd_t<D, Fp16>(a, p, s);
 }
 
 }  // namespace fa

@@ -12,7 +12,16 @@ int win_shape_rows(WinShape s);      // packed rows per workgroup
 int win_shape_groups(WinShape s);
 int win_shape_keys(WinShape s);      // keys per tile
 template <int D> hipError_t launch_window_fwd(const WinFwdArgs &a, int dtype, bool paged, WinShape shape, hipStream_t s);
-template <int D> hipError_t launch_window_bwd(const WinBwdArgs &a, int dtype, int max_rows, int max_k, hipStream_t s);
+
+// dense forward: waves of 32 packed rows to a workgroup, keys to a tile
+constexpr int WIN_FWD_WAVES = 4, WIN_FWD_KEYS = 64;
+// backward: waves of 32 packed rows (dQ), blocks of 32 keys and waves (dK, dV) to a workgroup
+constexpr int WIN_DQ_WAVES = 4, WIN_DKV_BLOCKS = 4;
+constexpr int win_dkv_waves(int D) { return D == 128 ? 2 * WIN_DKV_BLOCKS : WIN_DKV_BLOCKS; }
+struct WinBwdPlan {
+    int max_rows, max_k, order;
+};
+template <int D> hipError_t launch_window_bwd(const WinBwdArgs &a, int dtype, const WinBwdPlan &p, hipStream_t s);
 // the error text of the C ABI (fa_api.cpp)
 int set_error(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 void clear_error();

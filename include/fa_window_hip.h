@@ -34,7 +34,6 @@ typedef struct FaWindowArgs {
     /* backward only */
     const void *dout;             /* (total_q, nheads, head_dim) */
     void *dq, *dk, *dv;           /* outputs, shapes of q, k, v */
-    float *softmax_d;             /* (batch, nheads, lse_stride): rowsum(dout * o) */
     void *workspace;              /* fa_window_bwd_workspace() bytes, 16-byte aligned, any contents */
     int64_t workspace_bytes;
     int64_t q_row_stride, q_head_stride;
