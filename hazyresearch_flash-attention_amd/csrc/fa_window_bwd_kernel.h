@@ -13,7 +13,7 @@
 // keys but shows where a row sees few; there it is summed from P and dP in fp32 first (WIN_EXACT_TILES).
 #pragma once
 
-#include "fa_window_common.h"
+#include "fa_window_careful.h"
 
 namespace fa {
 
@@ -253,6 +253,29 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
     if (hi == 0 && row < R) a.ws_rows[rows_base(a, q_start, sq, kvh) + row] = f32x2{lse2, -delta};
     walk_all(std::false_type{});
 
+    // an infinity or NaN: this wave's rows again, key by key (fa_window_careful.h)
+    if (!all_finite(dq, 0.f)) {
+        LaneRow<D> qv, dv, kv, vv, acc;
+        for (int rr = 0; rr < 32 && rw + rr < R; ++rr) {
+            const int tt = a.dgroup.div(rw + rr), hh = kvh * G + rw + rr - tt * G, p = off + tt;
+            qv.template load<T>(a.q + (int64_t)(q_start + tt) * a.q_rs + (int64_t)hh * a.q_hs, head_dim);
+            dv.template load<T>(a.dout + (int64_t)(q_start + tt) * a.do_rs + (int64_t)hh * a.do_hs, head_dim);
+            const float l2 = __shfl(lse2, rr), del = __shfl(delta, rr);
+            acc.zero();
+            for (int n = 0; n < walk.n; ++n)
+                for (int j0 = walk.tile(n) * C::BN, st = 0; st < 2; ++st, j0 += 32) {
+                    uint32_t bits = seen_bits(j0, p, a.window, a.sinks) & bits_below(klen - j0);
+                    while (bits) {
+                        const int j = j0 + __builtin_ctz(bits);
+                        bits &= bits - 1;
+                        kv.template load<T>(kbase + (int64_t)j * a.k_rs, head_dim);
+                        vv.template load<T>(vbase + (int64_t)j * a.v_rs, head_dim);
+                        acc.add(fast_exp2(fmaf(qv.dot(kv), c_log2, -l2)) * (dv.dot(vv) - del), kv);
+                    }
+                }
+            acc.put(dq, rr);
+        }
+    }
     zero_tail(a.dq, a.dq_rs, a.dq_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
     store_rows<D, T>(dq, a.scale, smem + wave * 64 * D, head_dim, [&](int r) __attribute__((always_inline)) -> uint16_t * {
         if (rw + r >= R) return nullptr;
@@ -387,7 +410,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
     const int64_t key_w = ((int64_t)key - off + a.window) * G;                 // first row behind its window
     const int key_up = key_w < r_end && !(key < a.sinks && !split) ? (int)key_w : r_end;
     const int lane_beg = sink ? (key_w > r_end ? r_end : (int)key_w) : key_lo;
-    const int lane_end = sink ? (key < a.sinks ? r_end : lane_beg) : key_up;
+    const int lane_end = key >= klen || (sink && key >= a.sinks) ? lane_beg : (sink ? r_end : key_up);   // (none: empty)
 
     // ---- staging of tile n: row r is token r / G of head kvh G + r % G; rows behind the last land as zeros
     const uint16_t *qbase = a.q + (int64_t)q_start * a.q_rs + (int64_t)kvh * G * a.q_hs;
@@ -506,7 +529,6 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
     auto mask_p = [&](int n, f32x16 &p) __attribute__((always_inline)) {
         const int rt = row_of(n);
         uint32_t m = bits_below(lane_end - rt) & ~bits_below(lane_beg - rt);
-        if (key >= klen) m = 0;
         if (__builtin_amdgcn_ballot_w64(m != 0xFFFFFFFFu) == 0) return;
         asm volatile("");
         m >>= 4 * hi;
@@ -679,6 +701,39 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         }
     }
 
+    // an infinity or NaN: the wave's sums again, row by row (fa_window_careful.h). A sink's chunk takes the tiles that
+    // its waves took.
+    bool finite = all_finite(dk, 0.f);
+    if constexpr (!PAIR) finite = finite && all_finite(dv, 0.f);
+    if (!finite) {
+        LaneRow<D> kv, vv, qv, dv_, gk, gv;
+        for (int rr = 0; rr < 32 && kw + rr < klen; ++rr) {
+            kv.template load<T>(a.k + (int64_t)(k_start + kw + rr) * a.k_rs + (int64_t)kvh * a.k_hs, head_dim);
+            vv.template load<T>(a.v + (int64_t)(k_start + kw + rr) * a.v_rs + (int64_t)kvh * a.v_hs, head_dim);
+            const int beg = __shfl(lane_beg, rr), end = __shfl(lane_end, rr);
+            gk.zero();
+            gv.zero();
+            for (int n = 0; n < nt; ++n) {
+                if (!takes(n)) continue;
+                const int rt = row_of(n);
+                for (int r = rt > beg ? rt : beg; r < end && r < rt + C::BR; ++r) {
+                    const int tt = a.dgroup.div(r), hh = kvh * G + r - tt * G;
+                    qv.template load<T>(a.q + (int64_t)(q_start + tt) * a.q_rs + (int64_t)hh * a.q_hs, head_dim);
+                    dv_.template load<T>(a.dout + (int64_t)(q_start + tt) * a.do_rs + (int64_t)hh * a.do_hs, head_dim);
+                    const f32x2 x = rows_g[r];
+                    const float p = fast_exp2(fmaf(qv.dot(kv), c_log2, -x[0]));
+                    gv.add(p, dv_);
+                    gk.add(p * (dv_.dot(vv) + x[1]), qv);
+                }
+            }
+            if constexpr (PAIR) {
+                (dswave ? gk : gv).put(dk, rr);
+            } else {
+                gk.put(dk, rr);
+                gv.put(dv, rr);
+            }
+        }
+    }
     tails();
     __syncthreads();       // the ring is free: rows go out through it
     auto store = [&](const f32x16 (&x)[D / 32], bool is_v) __attribute__((always_inline)) {

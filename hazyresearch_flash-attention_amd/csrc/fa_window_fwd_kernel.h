@@ -14,7 +14,7 @@
 // path, as does one with drafted tokens or a page that is not there.
 #pragma once
 
-#include "fa_window_common.h"
+#include "fa_window_careful.h"
 
 namespace fa {
 
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     float l_i = 0.f, m_thr = -INFINITY, mc = 0.f;   // m_thr: the tile maximum that moves m; mc = m * c_log2
     const float thr_raw = WIN_RESCALE / c_log2;
 
-    // keys j .. j+31 that this lane's row sees
-    auto seen = [&](int j, uint32_t there) __attribute__((always_inline)) -> uint32_t {
+    // keys j .. j+31 that a row at position `pos` (with the path `my_mask`) sees
+    auto seen_by = [&](int pos, const uint64_t *my_mask, int j, uint32_t there) __attribute__((always_inline)) -> uint32_t {
         uint32_t m = seen_bits(j, pos, a.window, a.sinks) & bits_below(klen - j);
         if constexpr (TREE) {
             const int d = j - off;                            // first drafted token of the word, if not negative
@@ -312,6 +312,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         if constexpr (PAGED) m &= ((there & 1) ? 0xFFFFu : 0u) | ((there & 2) ? 0xFFFF0000u : 0u);
         return m;
     };
+    auto seen = [&](int j, uint32_t there) __attribute__((always_inline)) -> uint32_t { return seen_by(pos, my_mask, j, there); };
 
     auto compute = [&](int j0, int buf, uint32_t there) __attribute__((always_inline)) {
         const char *kb = gsm + buf * C::TILE, *vb = gsm + (2 + buf) * C::TILE;
@@ -426,6 +427,55 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     for (int n = 0; n < steps; n += 2) {
         step(std::integral_constant<int, 0>(), n);
         if (n + 1 < steps) step(std::integral_constant<int, 1>(), n + 1);
+    }
+
+    // ---- an infinity or NaN: this wave's rows again over its own tiles, key by key (fa_window_careful.h)
+    if (!all_finite(o, l_i)) {
+        LaneRow<D> qv, kv, vv, acc;
+        for (int rr = 0; rr < 32 && rw + rr < R; ++rr) {
+            const int tt = a.dgroup.div(rw + rr), gg = rw + rr - tt * G;
+            qv.template load<T>(a.q + (int64_t)(q_start + tt) * a.q_rs + (int64_t)(kvh * G + gg) * a.q_hs, head_dim);
+            acc.zero();
+            const uint64_t *mask = nullptr;
+            int p = off + tt;
+            if constexpr (TREE) {
+                mask = a.tree + (int64_t)(q_start + tt) * a.tree_words;
+                p = off + depth_s[tt] - 1;
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int n = 0; n < steps; ++n) {
+                if (idx(n) >= i_end) break;
+                for (int j0 = walk.tile(idx(n)) * BN, st = 0; st < C::NS; ++st, j0 += 32) {
+                    uint32_t bits = seen_by(p, mask, j0, 3u);
+                    while (bits) {
+                        const int j = j0 + __builtin_ctz(bits);
+                        bits &= bits - 1;
+                        int64_t ko = (int64_t)j * a.k_rs, vo = (int64_t)j * a.v_rs;
+                        if constexpr (PAGED) {
+                            const int e = tbl[j >> a.page_shift];
+                            if ((uint32_t)e >= (uint32_t)a.num_pages) continue;
+                            const int in = j & ((1 << a.page_shift) - 1);
+                            ko = (int64_t)e * a.k_ps + (int64_t)in * a.k_rs;
+                            vo = (int64_t)e * a.v_ps + (int64_t)in * a.v_rs;
+                        }
+                        kv.template load<T>(kbase + ko, head_dim);
+                        vv.template load<T>(vbase + vo, head_dim);
+                        const float s = qv.dot(kv) * a.scale * LOG2E;
+                        const float top = fmaxf(m, s);
+                        const float w0 = m == -INFINITY ? 0.f : fast_exp2(m - top), w1 = fast_exp2(s - top);
+                        l = l * w0 + w1;
+#pragma unroll
+                        for (int e = 0; e < LaneRow<D>::E; ++e) acc.x[e] = (m == -INFINITY ? 0.f : acc.x[e] * w0) + w1 * vv.x[e];
+                        m = top;
+                    }
+                }
+            }
+            acc.put(o, rr);
+            if (l32 == rr) {
+                m_thr = mc = m;
+                l_i = hi ? 0.f : l;
+            }
+        }
     }
 
     zero_tail(a.o, a.o_rs, a.o_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);

@@ -57,8 +57,8 @@ def flash_paged_attn_func(q, k_pages, v_pages, block_table, context_lens, cu_seq
     a capture for later lengths wants a bound on those. tree_mask (total_q, words) int64, 1 to 4 words, see above.
     window_size, num_sinks, softmax_scale and return_lse as in `flash_window_attn_unpadded_func`.
 
-    A table entry outside [0, num_pages) is not read: nobody sees its keys. Rows of a page behind the last key may
-    hold anything; keys in front of it have to be finite.
+    A table entry outside [0, num_pages) is not read: nobody sees its keys. Rows of a page that no token sees may hold
+    anything, infinities and NaN among them.
     """
     window, sinks = _window(window_size, num_sinks)
     r = _binding().paged_attn(q, k_pages, v_pages, block_table, context_lens, cu_seqlens_q, max_seqlen_q,

@@ -44,7 +44,8 @@ def flash_window_attn_unpadded_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seq
     Returns out (total_q, nheads, headdim), or (out, lse) with return_lse: lse (batch, nheads,
     round16(max_seqlen_q)) fp32, natural logarithm, without a gradient; entries past a sequence's end are unset.
 
-    Values of keys that a query does not see have to be finite all the same: their weight is 0, and 0 * inf is NaN.
+    An infinity or NaN reaches the results of what sees it and nothing else, forward and backward (rows whose tiles
+    hold one are computed again key by key, which is slow).
     """
     window, sinks = _window(window_size, num_sinks)
     out, lse = _binding().window_attn(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks,
