@@ -127,16 +127,15 @@ std::vector<at::Tensor> window_fwd(const at::Tensor &q_, const at::Tensor &k_, c
     return {o, lse};
 }
 
-std::vector<at::Tensor> window_bwd(const at::Tensor &dout_, const at::Tensor &q_, const at::Tensor &k_,
-                                   const at::Tensor &v_, const at::Tensor &o, const at::Tensor &lse,
-                                   const at::Tensor &cu_q, const at::Tensor &cu_k, int64_t max_q, int64_t max_k,
-                                   int64_t window, int64_t sinks, double scale) {
+// Writes dq, dk, dv (whole tensors or views of a packed one).
+void window_bwd(const at::Tensor &dout_, const at::Tensor &q_, const at::Tensor &k_, const at::Tensor &v_,
+                const at::Tensor &o, const at::Tensor &lse, at::Tensor dq, at::Tensor dk, at::Tensor dv,
+                const at::Tensor &cu_q, const at::Tensor &cu_k, int64_t max_q, int64_t max_k, int64_t window,
+                int64_t sinks, double scale) {
     TORCH_CHECK(dout_.sizes() == q_.sizes() && dout_.scalar_type() == q_.scalar_type() && dout_.device() == q_.device(),
                 "dout must have the shape, dtype and device of q");
     c10::DeviceGuard guard(q_.device());
     const at::Tensor q = rows(q_), k = rows(k_), v = rows(v_), dout = rows(dout_);
-    const auto dense = [](const at::Tensor &t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); };
-    at::Tensor dq = dense(q), dk = dense(k), dv = dense(v);
     if (max_q == 0) dq.zero_();
     if (max_k == 0) {
         dk.zero_();
@@ -160,8 +159,26 @@ std::vector<at::Tensor> window_bwd(const at::Tensor &dout_, const at::Tensor &q_
         a.workspace_bytes = bytes;
     }
     check_rc(fa_window_bwd(&a, stream_of(q)), "fa_window_bwd");
-    return {dq, dk, dv};
 }
+
+at::Tensor dense_like(const at::Tensor &t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); }
+
+struct WindowCfg {
+    int64_t max_q, max_k, window, sinks;
+    double scale;
+    void save(AutogradContext *ctx) const {
+        ctx->saved_data["mq"] = max_q;
+        ctx->saved_data["mk"] = max_k;
+        ctx->saved_data["w"] = window;
+        ctx->saved_data["n"] = sinks;
+        ctx->saved_data["sc"] = scale;
+    }
+    static WindowCfg load(AutogradContext *ctx) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "the windowed attention has no second derivative (create_graph=True)");
+        return {ctx->saved_data["mq"].toInt(), ctx->saved_data["mk"].toInt(), ctx->saved_data["w"].toInt(),
+                ctx->saved_data["n"].toInt(), ctx->saved_data["sc"].toDouble()};
+    }
+};
 
 struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
     static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &k, const at::Tensor &v,
@@ -170,24 +187,87 @@ struct WindowAttnFn : public torch::autograd::Function<WindowAttnFn> {
         auto r = window_fwd(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, scale);
         ctx->save_for_backward({q, k, v, r[0], r[1], cu_q, cu_k});
         ctx->mark_non_differentiable({r[1]});
-        ctx->saved_data["mq"] = max_q;
-        ctx->saved_data["mk"] = max_k;
-        ctx->saved_data["w"] = window;
-        ctx->saved_data["n"] = sinks;
-        ctx->saved_data["sc"] = scale;
+        WindowCfg{max_q, max_k, window, sinks, scale}.save(ctx);
         return {r[0], r[1]};
     }
     static variable_list backward(AutogradContext *ctx, variable_list g) {
-        TORCH_CHECK(!at::GradMode::is_enabled(), "flash_window_attn_unpadded_func has no second derivative (create_graph=True)");
-        auto t = ctx->get_saved_variables();
+        const WindowCfg c = WindowCfg::load(ctx);
         at::Tensor n;
         if (!g[0].defined()) return {n, n, n, n, n, n, n, n, n, n};
-        auto r = window_bwd(g[0], t[0], t[1], t[2], t[3], t[4], t[5], t[6], ctx->saved_data["mq"].toInt(),
-                            ctx->saved_data["mk"].toInt(), ctx->saved_data["w"].toInt(), ctx->saved_data["n"].toInt(),
-                            ctx->saved_data["sc"].toDouble());
-        return {r[0], r[1], r[2], n, n, n, n, n, n, n};
+        auto t = ctx->get_saved_variables();
+        c10::DeviceGuard guard(t[0].device());
+        at::Tensor dq = dense_like(t[0]), dk = dense_like(t[1]), dv = dense_like(t[2]);
+        window_bwd(g[0], t[0], t[1], t[2], t[3], t[4], dq, dk, dv, t[5], t[6], c.max_q, c.max_k, c.window, c.sinks, c.scale);
+        return {dq, dk, dv, n, n, n, n, n, n, n};
     }
 };
+
+// kv (total_k, 2, nheads_k, headdim): dkv written whole
+struct WindowAttnKVFn : public torch::autograd::Function<WindowAttnKVFn> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &q, const at::Tensor &kv, const at::Tensor &cu_q,
+                                 const at::Tensor &cu_k, int64_t max_q, int64_t max_k, int64_t window, int64_t sinks,
+                                 double scale) {
+        auto r = window_fwd(q, kv.select(1, 0), kv.select(1, 1), cu_q, cu_k, max_q, max_k, window, sinks, scale);
+        ctx->save_for_backward({q, kv, r[0], r[1], cu_q, cu_k});
+        ctx->mark_non_differentiable({r[1]});
+        WindowCfg{max_q, max_k, window, sinks, scale}.save(ctx);
+        return {r[0], r[1]};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const WindowCfg c = WindowCfg::load(ctx);
+        at::Tensor n;
+        if (!g[0].defined()) return {n, n, n, n, n, n, n, n, n};
+        auto t = ctx->get_saved_variables();
+        c10::DeviceGuard guard(t[0].device());
+        at::Tensor dq = dense_like(t[0]), dkv = dense_like(t[1]);
+        window_bwd(g[0], t[0], t[1].select(1, 0), t[1].select(1, 1), t[2], t[3], dq, dkv.select(1, 0), dkv.select(1, 1),
+                   t[4], t[5], c.max_q, c.max_k, c.window, c.sinks, c.scale);
+        return {dq, dkv, n, n, n, n, n, n, n};
+    }
+};
+
+// qkv (total, 3, nheads, headdim): dqkv written whole
+struct WindowAttnQKVFn : public torch::autograd::Function<WindowAttnQKVFn> {
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &qkv, const at::Tensor &cu, int64_t max_s,
+                                 int64_t window, int64_t sinks, double scale) {
+        auto r = window_fwd(qkv.select(1, 0), qkv.select(1, 1), qkv.select(1, 2), cu, cu, max_s, max_s, window, sinks, scale);
+        ctx->save_for_backward({qkv, r[0], r[1], cu});
+        ctx->mark_non_differentiable({r[1]});
+        WindowCfg{max_s, max_s, window, sinks, scale}.save(ctx);
+        return {r[0], r[1]};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const WindowCfg c = WindowCfg::load(ctx);
+        at::Tensor n;
+        if (!g[0].defined()) return {n, n, n, n, n, n};
+        auto t = ctx->get_saved_variables();
+        c10::DeviceGuard guard(t[0].device());
+        at::Tensor d = dense_like(t[0]);
+        window_bwd(g[0], t[0].select(1, 0), t[0].select(1, 1), t[0].select(1, 2), t[1], t[2], d.select(1, 0), d.select(1, 1),
+                   d.select(1, 2), t[3], t[3], c.max_q, c.max_k, c.window, c.sinks, c.scale);
+        return {d, n, n, n, n, n};
+    }
+};
+
+std::vector<at::Tensor> window_attn_kv(const at::Tensor &q, const at::Tensor &kv, const at::Tensor &cu_q, const at::Tensor &cu_k,
+                                       int64_t max_q, int64_t max_k, int64_t window, int64_t sinks,
+                                       c10::optional<double> scale_opt) {
+    TORCH_CHECK(q.dim() == 3, "q must be (total_q, nheads, headdim)");
+    TORCH_CHECK(kv.dim() == 4 && kv.size(1) == 2, "kv must be (total_k, 2, nheads, headdim)");
+    const double scale = scale_opt ? *scale_opt : 1.0 / std::sqrt((double)q.size(2));
+    if (!wants_grad(q) && !wants_grad(kv))
+        return window_fwd(q, kv.select(1, 0), kv.select(1, 1), cu_q, cu_k, max_q, max_k, window, sinks, scale);
+    return WindowAttnKVFn::apply(q, kv, cu_q, cu_k, max_q, max_k, window, sinks, scale);
+}
+
+std::vector<at::Tensor> window_attn_qkv(const at::Tensor &qkv, const at::Tensor &cu, int64_t max_s, int64_t window,
+                                        int64_t sinks, c10::optional<double> scale_opt) {
+    TORCH_CHECK(qkv.dim() == 4 && qkv.size(1) == 3, "qkv must be (total, 3, nheads, headdim)");
+    const double scale = scale_opt ? *scale_opt : 1.0 / std::sqrt((double)qkv.size(3));
+    if (!wants_grad(qkv))
+        return window_fwd(qkv.select(1, 0), qkv.select(1, 1), qkv.select(1, 2), cu, cu, max_s, max_s, window, sinks, scale);
+    return WindowAttnQKVFn::apply(qkv, cu, max_s, window, sinks, scale);
+}
 
 std::vector<at::Tensor> window_attn(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &cu_q,
                                     const at::Tensor &cu_k, int64_t max_q, int64_t max_k, int64_t window, int64_t sinks,
@@ -402,6 +482,8 @@ struct Cache {
 
 void bind_window(pybind11::module &m) {
     m.def("window_attn", &window_attn);
+    m.def("window_attn_kv", &window_attn_kv);
+    m.def("window_attn_qkv", &window_attn_qkv);
     m.def("paged_attn", &paged_attn);
     pybind11::class_<Cache>(m, "PagedCache")
         .def(pybind11::init<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, int64_t, int64_t>())

@@ -9,6 +9,7 @@ import torch.nn as nn
 
 from flash_attn.bert_padding import pad_input, unpad_input
 from flash_attn.flash_attn_interface import flash_attn_unpadded_qkvpacked_func
+from flash_attn.flash_window_attn_interface import flash_window_attn_unpadded_qkvpacked_func
 from flash_attn.rotary import RotaryEmbedding, RotaryEmbedding2D, apply_rotary_emb_qkv_
 
 
@@ -16,12 +17,26 @@ class FlashAttention(nn.Module):
     """Scaled dot-product attention with softmax over packed qkv.
 
     softmax_scale: temperature (default 1/sqrt(headdim)); attention_dropout: dropout rate in
-    training mode."""
+    training mode. window_size, num_sinks: a causal token sees the window_size newest tokens, itself
+    among them, and the first num_sinks (flash_window_attn_interface); no dropout then."""
 
-    def __init__(self, softmax_scale=None, attention_dropout=0.0, device=None, dtype=None):
+    def __init__(self, softmax_scale=None, attention_dropout=0.0, device=None, dtype=None, window_size=None,
+                 num_sinks=0):
         super().__init__()
         self.softmax_scale = softmax_scale
         self.dropout_p = attention_dropout
+        self.window_size, self.num_sinks = window_size, num_sinks
+        if window_size is not None and attention_dropout > 0.0:
+            raise RuntimeError("a windowed attention has no dropout")
+
+    def _attend(self, qkv, cu_seqlens, max_s, dropout_p, causal):
+        if self.window_size is None:
+            return flash_attn_unpadded_qkvpacked_func(qkv, cu_seqlens, max_s, dropout_p,
+                                                      softmax_scale=self.softmax_scale, causal=causal)
+        if not causal or dropout_p > 0.0:
+            raise RuntimeError("a windowed attention is causal and has no dropout")
+        return flash_window_attn_unpadded_qkvpacked_func(qkv, cu_seqlens, max_s, self.window_size, self.num_sinks,
+                                                         softmax_scale=self.softmax_scale)
 
     def forward(self, qkv, key_padding_mask=None, causal=False, cu_seqlens=None, max_s=None,
                 need_weights=False):
@@ -33,22 +48,18 @@ class FlashAttention(nn.Module):
         dropout_p = self.dropout_p if self.training else 0.0
         if cu_seqlens is not None:
             assert max_s is not None
-            out = flash_attn_unpadded_qkvpacked_func(qkv, cu_seqlens, max_s, dropout_p,
-                                                     softmax_scale=self.softmax_scale, causal=causal)
-            return out, None
+            return self._attend(qkv, cu_seqlens, max_s, dropout_p, causal), None
         batch, seqlen = qkv.shape[0], qkv.shape[1]
         if key_padding_mask is None:
             qkv_u = qkv.reshape(batch * seqlen, *qkv.shape[2:])
             cu = torch.arange(0, (batch + 1) * seqlen, seqlen, dtype=torch.int32, device=qkv.device)
-            out = flash_attn_unpadded_qkvpacked_func(qkv_u, cu, seqlen, dropout_p,
-                                                     softmax_scale=self.softmax_scale, causal=causal)
+            out = self._attend(qkv_u, cu, seqlen, dropout_p, causal)
             return out.reshape(batch, seqlen, *out.shape[1:]), None
         nheads = qkv.shape[-2]
         x = qkv.reshape(batch, seqlen, -1)
         x_u, indices, cu, max_s = unpad_input(x, key_padding_mask)
         x_u = x_u.reshape(x_u.shape[0], 3, nheads, -1)
-        out_u = flash_attn_unpadded_qkvpacked_func(x_u, cu, max_s, dropout_p,
-                                                   softmax_scale=self.softmax_scale, causal=causal)
+        out_u = self._attend(x_u, cu, max_s, dropout_p, causal)
         out = pad_input(out_u.reshape(out_u.shape[0], -1), indices, batch, seqlen)
         return out.reshape(batch, seqlen, nheads, -1), None
 
@@ -169,11 +180,15 @@ def _uniform_cu_seqlens(B, S, device):
 
 
 class FlashMHA(nn.Module):
-    """Multi-head attention block: Wqkv -> optional rotary -> FlashAttention -> out_proj."""
+    """Multi-head attention block: Wqkv -> optional rotary -> FlashAttention -> out_proj. window_size,
+    num_sinks (causal, no dropout): as in FlashAttention."""
 
     def __init__(self, embed_dim, num_heads, bias=True, batch_first=True, attention_dropout=0.0,
-                 causal=False, use_rotary_emb=None, device=None, dtype=None, **kwargs) -> None:
+                 causal=False, use_rotary_emb=None, device=None, dtype=None, window_size=None, num_sinks=0,
+                 **kwargs) -> None:
         assert batch_first
+        if window_size is not None and not causal:
+            raise RuntimeError("a windowed attention is causal")
         factory_kwargs = {"device": device, "dtype": dtype}
         super().__init__()
         self.embed_dim = embed_dim
@@ -189,14 +204,15 @@ class FlashMHA(nn.Module):
         elif use_rotary_emb == "2d":
             self.rotary_emb = RotaryEmbedding2D(self.head_dim)
         self.Wqkv = nn.Linear(embed_dim, 3 * embed_dim, bias=bias, **factory_kwargs)
-        self.inner_attn = FlashAttention(attention_dropout=attention_dropout, **factory_kwargs)
+        self.inner_attn = FlashAttention(attention_dropout=attention_dropout, window_size=window_size,
+                                         num_sinks=num_sinks, **factory_kwargs)
         self.out_proj = nn.Linear(embed_dim, embed_dim, bias=bias, **factory_kwargs)
 
     def forward(self, x, key_padding_mask=None, need_weights=False):
         """x: (batch, seqlen, embed_dim); key_padding_mask: (batch, seqlen) bool."""
         qkv = self.Wqkv(x)
         b, s = qkv.shape[0], qkv.shape[1]
-        fused = (self.use_rotary_emb and qkv.is_cuda and qkv.is_contiguous() and key_padding_mask is None
+        fused = (self.use_rotary_emb and self.inner_attn.window_size is None and qkv.is_cuda and qkv.is_contiguous() and key_padding_mask is None
                  and qkv.dtype in (torch.float16, torch.bfloat16) and self.head_dim % 8 == 0)
         if fused:
             cos, sin = self.rotary_emb.cos_sin_tables(s, qkv.device, qkv.dtype)

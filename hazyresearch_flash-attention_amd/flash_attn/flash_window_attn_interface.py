@@ -51,3 +51,20 @@ def flash_window_attn_unpadded_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seq
     out, lse = _binding().window_attn(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks,
                                       softmax_scale)
     return (out, lse) if return_lse else out
+
+
+def flash_window_attn_unpadded_kvpacked_func(q, kv, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
+                                             window_size=None, num_sinks=0, softmax_scale=None, return_lse=False):
+    """`flash_window_attn_unpadded_func` of q (total_q, nheads, headdim) over packed kv (total_k, 2, nheads_k, headdim)."""
+    window, sinks = _window(window_size, num_sinks)
+    out, lse = _binding().window_attn_kv(q, kv, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks,
+                                         softmax_scale)
+    return (out, lse) if return_lse else out
+
+
+def flash_window_attn_unpadded_qkvpacked_func(qkv, cu_seqlens, max_seqlen, window_size=None, num_sinks=0,
+                                              softmax_scale=None, return_lse=False):
+    """`flash_window_attn_unpadded_func` of packed qkv (total, 3, nheads, headdim)."""
+    window, sinks = _window(window_size, num_sinks)
+    out, lse = _binding().window_attn_qkv(qkv, cu_seqlens, max_seqlen, window, sinks, softmax_scale)
+    return (out, lse) if return_lse else out

@@ -409,3 +409,61 @@ def test_nothing_to_do(n):
     assert out.shape == q.shape and not out.any()
     dq, dk = torch.autograd.grad(out, (q, k), torch.ones_like(out))
     assert not dq.any() and not dk.any()
+
+
+@pytest.mark.gpu
+def test_packed_forms():
+    """kvpacked and qkvpacked: the separate form's outputs and gradients, bit for bit."""
+    from flash_attn import flash_window_attn_interface as fw
+    from window_testutil import cu, randn
+    c = cu([90, 1, 40])
+    qkv = randn(0, (150, 3, 4, 64), torch.bfloat16).requires_grad_()
+    dout = randn(1, (150, 4, 64), torch.bfloat16)
+    q, k, v = (qkv.detach()[:, i].clone().requires_grad_() for i in range(3))
+    want = fw.flash_window_attn_unpadded_func(q, k, v, c, c, 90, 90, 20, 2)
+    grads = torch.stack(torch.autograd.grad(want, (q, k, v), dout), 1)
+    out, lse = fw.flash_window_attn_unpadded_qkvpacked_func(qkv, c, 90, 20, 2, return_lse=True)
+    assert lse.shape == (3, 4, 96) and not lse.requires_grad
+    assert torch.equal(out, want) and torch.equal(torch.autograd.grad(out, qkv, dout)[0], grads)
+    kv = qkv.detach()[:, 1:].clone().requires_grad_()
+    out = fw.flash_window_attn_unpadded_kvpacked_func(q, kv, c, c, 90, 90, 20, 2)
+    dq, dkv = torch.autograd.grad(out, (q, kv), dout)
+    assert torch.equal(out, want) and torch.equal(dq, grads[:, 0]) and torch.equal(dkv, grads[:, 1:])
+    with pytest.raises(RuntimeError, match="qkv must be"):
+        fw.flash_window_attn_unpadded_qkvpacked_func(kv, c, 90, 20)
+
+
+def test_modules_refuse_a_window_without_its_mask():
+    from flash_attn.flash_attention import FlashAttention, FlashMHA
+    with pytest.raises(RuntimeError, match="dropout"):
+        FlashAttention(attention_dropout=0.1, window_size=8)
+    with pytest.raises(RuntimeError, match="causal"):
+        FlashMHA(64, 2, window_size=8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotary", [None, "1d"])
+def test_modules(rotary):
+    """FlashMHA with a window, padded and not, against its own unwindowed layers around the plain form; gradients run."""
+    from flash_attn.flash_attention import FlashAttention, FlashMHA
+    from oracle import window_ref as ref
+    torch.manual_seed(0)
+    m = FlashMHA(128, 2, causal=True, use_rotary_emb=rotary, window_size=9, num_sinks=2, device="cuda", dtype=torch.bfloat16)
+    x = torch.randn(2, 50, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    mask = torch.ones(2, 50, dtype=torch.bool, device="cuda")
+    mask[1, 30:] = False
+    full, _ = m(x)
+    padded, _ = m(x, key_padding_mask=mask)
+    assert torch.equal(full[0], padded[0]) and torch.equal(full[1, :30], padded[1, :30])
+    full.float().square().sum().backward()
+    assert torch.isfinite(x.grad).all() and x.grad.abs().sum() > 0
+    inner = FlashAttention(window_size=9, num_sinks=2)
+    qkv = torch.randn(1, 50, 3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    out, _ = inner(qkv, causal=True)
+    live = ref.seen(torch.arange(50, device="cuda"), torch.arange(50, device="cuda"), 9, 2)
+    for h in range(2):
+        a = (*(qkv[0, :, i, h] for i in range(3)), live, 64 ** -0.5)
+        r, _, p = ref.attention(*a)
+        assert ((out[0, :, h].double() - r).abs() <= ref.bounds(*a, p, r)).all()
+    with pytest.raises(RuntimeError, match="causal"):
+        inner(qkv)
