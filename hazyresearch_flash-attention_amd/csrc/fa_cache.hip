@@ -38,135 +38,136 @@ __device__ void release(const FaCache &c, int32_t *tbl, int from, int to) {
     }
 }
 
-// exclusive prefix sum of one value per thread over a workgroup of 1024; total to all
-__device__ int scan1024(int v, int *tmp /* 17 words */, int &total) {
+// exclusive prefix sums of one value per thread over a workgroup of 1024; total to all. tmp: 16 words, free again after
+// the next barrier
+template <typename V>
+__device__ V scan1024(V v, V *tmp, V &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
+    V x = v;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-        const int y = __shfl_up(x, s);
+        const V y = __shfl_up(x, s);
         if (lane >= s) x += y;
     }
-    __syncthreads();
     if (lane == 63) tmp[wave] = x;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int run = 0;
-        for (int i = 0; i < 16; ++i) {
-            const int y = tmp[i];
-            tmp[i] = run;
-            run += y;
-        }
-        tmp[16] = run;
+    V before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const V y = tmp[i];
+        before += i < wave ? y : 0;
+        all += y;
     }
-    __syncthreads();
-    total = tmp[16];
-    return tmp[wave] + x - v;
+    total = all;
+    return before + x - v;
 }
 
 // One workgroup: what each slot needs, the lowest free pages that cover it, then the tables. Nothing is written to
-// them before all is known to fit.
+// them before all is known to fit. Bound by the chain of dependent loads (slots, lengths, entries, counts), so the first
+// 4096 pages' counts are on their way from the start, and each thread keeps its slots in registers.
+constexpr int RES_PER = FA_CACHE_MAX_SLOTS / 1024;
 __global__ __launch_bounds__(1024) void cache_reserve_kernel(const FaCache c, const int32_t *slots, int n,
                                                              const int32_t *counts, int count) {
     __shared__ uint32_t named[FA_CACHE_MAX_SEQS / 32];
-    __shared__ int shared_page[FA_CACHE_MAX_SLOTS];      // a partly full page that others hold too, or -1
-    __shared__ int first[FA_CACHE_MAX_SLOTS];            // rank of the slot's first new page
-    __shared__ uint8_t copies[FA_CACHE_MAX_SLOTS];
-    __shared__ int tmp[17];
-    const int tid = threadIdx.x, ps = c.page_size;
-    constexpr int PER = FA_CACHE_MAX_SLOTS / 1024;
-    if (tid == 0) c.scratch[SCR_COPIES] = 0;
-    for (int i = tid; i < FA_CACHE_MAX_SEQS / 32; i += 1024) named[i] = 0;
-    __syncthreads();
-    int bad = 0, len[PER], cnt[PER], have[PER], slot[PER];
-    const int per = (n + 1023) / 1024;                   // consecutive slots to a thread
+    __shared__ __attribute__((aligned(16))) int shared_page[FA_CACHE_MAX_SLOTS];      // a partly full page that others hold too, or -1
+    __shared__ int sbad;
+    __shared__ long long tmp[2][16];
+    __shared__ int tmp32[2][16];
+    const int tid = threadIdx.x, lane = tid & 63, ps = c.page_size;
+    auto free_at = [&](int p) -> bool { return p < c.num_pages && c.refcount[p] == 0; };
+    bool is_free[4];
 #pragma unroll
-    for (int x = 0; x < PER; ++x) {
+    for (int x = 0; x < 4; ++x) is_free[x] = free_at(tid * 4 + x);
+    const int per = (n + 1023) / 1024;                   // consecutive slots to a thread
+    int slot[RES_PER], cnt[RES_PER];
+#pragma unroll
+    for (int x = 0; x < RES_PER; ++x) {
         const int i = tid * per + x;
-        slot[x] = -1;
-        len[x] = cnt[x] = have[x] = 0;
-        if (x >= per || i >= n) continue;
-        shared_page[i] = -1;
-        const int s = slots[i];
+        slot[x] = x < per && i < n ? slots[i] : -1;
+        cnt[x] = x < per && i < n && counts ? counts[i] : count;
+    }
+    if (tid == 0) {
+        c.scratch[SCR_COPIES] = 0;
+        sbad = 0;
+    }
+    for (int i = tid; i < FA_CACHE_MAX_SEQS / 32; i += 1024) named[i] = 0;
+    for (int i = tid; i < FA_CACHE_MAX_SLOTS; i += 1024) shared_page[i] = -1;
+    __syncthreads();
+    int bad = 0, len[RES_PER], have[RES_PER], page[RES_PER], refs[RES_PER];
+#pragma unroll
+    for (int x = 0; x < RES_PER; ++x) {
+        const int s = slot[x];
+        len[x] = have[x] = refs[x] = 0;
+        page[x] = -1;
         if (s == -1) continue;
+        slot[x] = -1;
         if (s < 0 || s >= c.max_seqs || (atomicOr(&named[s >> 5], 1u << (s & 31)) >> (s & 31) & 1)) {
             bad |= FA_CACHE_BAD_SLOT;
-            continue;
-        }
-        const int m = counts ? counts[i] : count;
-        if (m < 0) {
+        } else if (cnt[x] < 0) {
             bad |= FA_CACHE_BAD_LENGTH;
-            continue;
-        }
-        if (m == 0) continue;
-        slot[x] = s;
-        len[x] = c.seqlens[s];
-        cnt[x] = m;
-        have[x] = c.nblocks[s];
-        if (((int64_t)len[x] + m + ps - 1) / ps > c.max_blocks) {
-            bad |= FA_CACHE_TOO_LONG;
-            slot[x] = -1;
-            continue;
-        }
-        if (len[x] % ps) {
-            const int page = c.block_table[(int64_t)s * c.max_blocks + len[x] / ps];
-            if (page < 0 || page >= c.num_pages)
-                bad |= FA_CACHE_NOT_RESERVED;            // the last token's page was given back
-            else if (c.refcount[page] > 1)
-                shared_page[i] = page;
+        } else if (cnt[x] > 0) {
+            len[x] = c.seqlens[s];
+            have[x] = c.nblocks[s];
+            if (((int64_t)len[x] + cnt[x] + ps - 1) / ps > c.max_blocks) {
+                bad |= FA_CACHE_TOO_LONG;
+                continue;
+            }
+            slot[x] = s;
+            if (len[x] % ps) {
+                const int p = c.block_table[(int64_t)s * c.max_blocks + len[x] / ps];
+                if (p < 0 || p >= c.num_pages) {
+                    bad |= FA_CACHE_NOT_RESERVED;        // the last token's page was given back
+                } else if ((refs[x] = c.refcount[p]) > 1) {
+                    page[x] = p;
+                    shared_page[tid * per + x] = p;
+                }
+            }
         }
     }
-    bad = (__syncthreads_or(bad & FA_CACHE_BAD_SLOT) ? FA_CACHE_BAD_SLOT : 0) |
-          (__syncthreads_or(bad & FA_CACHE_BAD_LENGTH) ? FA_CACHE_BAD_LENGTH : 0) |
-          (__syncthreads_or(bad & FA_CACHE_TOO_LONG) ? FA_CACHE_TOO_LONG : 0) |
-          (__syncthreads_or(bad & FA_CACHE_NOT_RESERVED) ? FA_CACHE_NOT_RESERVED : 0);
-    if (bad) {
-        if (tid == 0) flag(c, bad);
+    if (bad) atomicOr(&sbad, bad);
+    __syncthreads();
+    if (sbad) {
+        if (tid == 0) flag(c, sbad);
         return;
     }
-    int mine = 0, mycopies = 0;
-    int need[PER];
+    // a shared page is copied unless this is its last holder: earlier slots of the call leave it first
+    long long mine = 0;                                  // pages needed, and copies above them
+    int need[RES_PER];
+    bool copy[RES_PER];
 #pragma unroll
-    for (int x = 0; x < PER; ++x) {
+    for (int x = 0; x < RES_PER; ++x) {
         const int i = tid * per + x;
         need[x] = 0;
-        if (x >= per || i >= n) continue;
-        bool copy = false;
-        if (shared_page[i] >= 0) {
-            int before = 0;                              // earlier slots of the call that leave the page
-            for (int j = 0; j < i; ++j) before += shared_page[j] == shared_page[i];
-            copy = c.refcount[shared_page[i]] - before > 1;
-        }
-        copies[i] = copy;
-        if (slot[x] >= 0) {
-            const int more = blocks_of((int64_t)len[x] + cnt[x], ps) - have[x];
-            need[x] = (copy ? 1 : 0) + (more > 0 ? more : 0);
-        }
-        mine += need[x];
-        mycopies += copy;
-    }
-    int total, ncopies;
-    int rank = scan1024(mine, tmp, total);
-    const int copy_rank = scan1024(mycopies, tmp, ncopies);
+        copy[x] = false;
+        if (slot[x] < 0) continue;
+        if (page[x] >= 0) {
+            int before = 0;
+            typedef int i32x4s __attribute__((ext_vector_type(4)));
+            for (int j = 0; j < i; j += 4) {
+                const i32x4s o = *(const i32x4s *)(shared_page + j);
 #pragma unroll
-    for (int x = 0; x < PER; ++x) {
-        const int i = tid * per + x;
-        if (x < per && i < n) first[i] = rank;
-        rank += need[x];
+                for (int e = 0; e < 4; ++e) before += j + e < i && o[e] == page[x];
+            }
+            copy[x] = refs[x] - before > 1;
+        }
+        const int more = blocks_of((int64_t)len[x] + cnt[x], ps) - have[x];
+        need[x] = (copy[x] ? 1 : 0) + (more > 0 ? more : 0);
+        mine += need[x] + ((long long)copy[x] << 32);
     }
+    long long sums;
+    const long long at0 = scan1024<long long>(mine, tmp[0], sums);
+    const int total = (int)sums, ncopies = (int)(sums >> 32);
     if (total == 0) return;
     // the `total` lowest free pages, in order
     int32_t *list = c.scratch + SCR_FREE;
     int found = 0;
-    for (int p0 = 0; p0 < c.num_pages && found < total; p0 += 4096) {
-        int is_free[4], f = 0;
+    for (int p0 = 0, round = 0; p0 < c.num_pages && found < total; p0 += 4096, round ^= 1) {
+        if (p0 > 0) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int p = p0 + tid * 4 + x;
-            is_free[x] = p < c.num_pages && c.refcount[p] == 0;
-            f += is_free[x];
+            for (int x = 0; x < 4; ++x) is_free[x] = free_at(p0 + tid * 4 + x);
         }
-        int here, at = found + scan1024(f, tmp, here);
+        const int f = (int)is_free[0] + is_free[1] + is_free[2] + is_free[3];
+        int here, at = found + scan1024<int>(f, tmp32[round], here);
 #pragma unroll
         for (int x = 0; x < 4; ++x)
             if (is_free[x]) {
@@ -180,50 +181,43 @@ __global__ __launch_bounds__(1024) void cache_reserve_kernel(const FaCache c, co
         return;
     }
     if (tid == 0) c.scratch[SCR_COPIES] = ncopies;
-    {
-        int at = copy_rank;
-#pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const int i = tid * per + x;
-            if (x < per && i < n && copies[i]) {
-                int32_t *e = c.scratch + SCR_LIST + 3 * at++;
-                e[0] = shared_page[i];
-                e[2] = len[x] % ps;
-            }
-        }
-    }
     __threadfence();
     __syncthreads();
-    // the tables: a thread sets what belongs to the slot, a wave deals out its new pages
-    {
-        int at = copy_rank;
+    // the tables: a thread sets its slots' copies and first new blocks, its wave the rest of long ones
+    constexpr int OWN = 4;
+    int rank = (int)at0, crank = (int)(at0 >> 32);
 #pragma unroll
-        for (int x = 0; x < PER; ++x) {
-            const int i = tid * per + x;
-            if (x >= per || i >= n || need[x] == 0) continue;
-            if (copies[i]) {
-                const int page = list[first[i]];
-                c.block_table[(int64_t)slot[x] * c.max_blocks + len[x] / ps] = page;
-                c.refcount[page] = 1;
-                atomicSub(c.refcount + shared_page[i], 1);
-                c.scratch[SCR_LIST + 3 * at++ + 1] = page;
+    for (int x = 0; x < RES_PER; ++x) {
+        const int64_t row = (int64_t)slot[x] * c.max_blocks;
+        if (copy[x]) {
+            const int p = list[rank++];
+            c.block_table[row + len[x] / ps] = p;
+            c.refcount[p] = 1;
+            atomicSub(c.refcount + page[x], 1);
+            int32_t *e = c.scratch + SCR_LIST + 3 * crank++;
+            e[0] = page[x];
+            e[1] = p;
+            e[2] = len[x] % ps;
+        }
+        const int more = need[x] - (copy[x] ? 1 : 0);
+        for (int b = 0; b < more && b < OWN; ++b) {
+            const int p = list[rank + b];
+            c.block_table[row + have[x] + b] = p;
+            c.refcount[p] = 1;
+        }
+        if (more > 0) c.nblocks[slot[x]] = have[x] + more;
+        uint64_t longer = __builtin_amdgcn_ballot_w64(more > OWN);
+        while (longer) {
+            const int src = __builtin_ctzll(longer);
+            longer &= longer - 1;
+            const int s = __shfl(slot[x], src), h = __shfl(have[x], src), m = __shfl(more, src), r = __shfl(rank, src);
+            for (int b = OWN + lane; b < m; b += 64) {
+                const int p = list[r + b];
+                c.block_table[(int64_t)s * c.max_blocks + h + b] = p;
+                c.refcount[p] = 1;
             }
         }
-    }
-    const int lane = tid & 63;
-    for (int i = tid >> 6; i < n; i += 16) {
-        const int s = slots[i];
-        if (s < 0) continue;
-        const int m = counts ? counts[i] : count;
-        if (m == 0) continue;
-        const int has = c.nblocks[s], end = blocks_of((int64_t)c.seqlens[s] + m, ps);
-        const int at = first[i] + copies[i];
-        for (int b = has + lane; b < end; b += 64) {
-            const int page = list[at + b - has];
-            c.block_table[(int64_t)s * c.max_blocks + b] = page;
-            c.refcount[page] = 1;
-        }
-        if (lane == 0 && end > has) c.nblocks[s] = end;
+        rank += more;
     }
 }
 
@@ -260,39 +254,60 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(const FaCache c) {
     }
 }
 
-// New rows into their pages: blockIdx.y the slot, a block takes `tok` tokens, lanes the row's 16-byte pieces.
+// New rows into their pages: blockIdx.y the slot; a block takes `lines` tokens at a time (a lane one 16-byte piece of
+// the row, in K and in V), WRITE_STEPS times, all loads before the first store: bound by HBM for long calls, by launch
+// and three dependent loads (length, table, row) for short ones.
+constexpr int WRITE_STEPS = 4;
 __global__ __launch_bounds__(256) void cache_write_kernel(const FaCache c, int layer, const int32_t *slots,
                                                           const uint16_t *k, int64_t k_rs, int64_t k_hs,
                                                           const uint16_t *v, int64_t v_rs, int64_t v_hs,
-                                                          const int32_t *cu, int64_t total, int tok) {
+                                                          const int32_t *cu, int64_t total, int lines) {
     const int i = blockIdx.y, s = slots[i];
+    int beg = cu[i], end = cu[i + 1];
     if (s == -1) return;
     if (s < 0 || s >= c.max_seqs) {
         if (threadIdx.x == 0 && blockIdx.x == 0) flag(c, FA_CACHE_BAD_SLOT);
         return;
     }
-    int beg = cu[i], end = cu[i + 1];
     beg = beg < 0 ? 0 : beg;
     end = end > total ? (int)total : end;
-    const int t0 = beg + blockIdx.x * tok;
-    const int t1 = end < t0 + tok ? end : t0 + tok;
-    if (t0 >= t1) return;
     const int hc = c.head_dim / 8, chunks = c.nheads * hc;
-    const int n = (t1 - t0) * chunks, len = c.seqlens[s], have = c.nblocks[s];
+    const int t0 = beg + blockIdx.x * lines * WRITE_STEPS;
+    if (t0 >= end) return;
+    const int len = c.seqlens[s], have = c.nblocks[s], shift = __builtin_ctz(c.page_size);
     const int64_t row = (int64_t)c.nheads * c.head_dim, layer0 = (int64_t)layer * c.num_pages * c.page_size * row;
-    for (int x = threadIdx.x; x < n; x += 256) {
-        const int t = t0 + x / chunks, ch = x % chunks, h = ch / hc, d = (ch - h * hc) * 8;
-        const int at = len + t - beg, blk = at / c.page_size;
-        const int page = at >= 0 && blk < have ? c.block_table[(int64_t)s * c.max_blocks + blk] : -1;
-        if (page < 0 || page >= c.num_pages || c.refcount[page] != 1) {
-            flag(c, FA_CACHE_NOT_RESERVED);
-            continue;
+    const int32_t *tbl = c.block_table + (int64_t)s * c.max_blocks;
+    // rows wider than a block: several pieces to a lane, one token at a time
+    for (int ch0 = 0; ch0 < chunks; ch0 += 256) {
+        const int line = lines > 1 ? threadIdx.x / chunks : 0;
+        const int ch = lines > 1 ? threadIdx.x - line * chunks : ch0 + threadIdx.x;
+        if (line >= lines || ch >= chunks) continue;
+        const int h = ch / hc, d = (ch - h * hc) * 8;
+        const uint16_t *kp = k + (int64_t)h * k_hs + d, *vp = v + (int64_t)h * v_hs + d;
+        u32x4v x[WRITE_STEPS], y[WRITE_STEPS];
+        int page[WRITE_STEPS];
+#pragma unroll
+        for (int n = 0; n < WRITE_STEPS; ++n) {
+            const int t = t0 + n * lines + line, at = len + t - beg, blk = at >> shift;
+            page[n] = -1;
+            if (t < end) {
+                page[n] = at >= 0 && blk < have ? tbl[blk] : -2;
+                x[n] = *(const u32x4v *)(kp + (int64_t)t * k_rs);
+                y[n] = *(const u32x4v *)(vp + (int64_t)t * v_rs);
+            }
         }
-        const int64_t dst = layer0 + ((int64_t)page * c.page_size + at % c.page_size) * row + h * c.head_dim + d;
-        const u32x4v a = *(const u32x4v *)(k + (int64_t)t * k_rs + (int64_t)h * k_hs + d);
-        const u32x4v b = *(const u32x4v *)(v + (int64_t)t * v_rs + (int64_t)h * v_hs + d);
-        *(u32x4v *)((uint16_t *)c.k_pages + dst) = a;
-        *(u32x4v *)((uint16_t *)c.v_pages + dst) = b;
+#pragma unroll
+        for (int n = 0; n < WRITE_STEPS; ++n) {
+            const int t = t0 + n * lines + line, at = len + t - beg;
+            if (t >= end) continue;
+            if (page[n] < 0 || page[n] >= c.num_pages || c.refcount[page[n]] != 1) {
+                flag(c, FA_CACHE_NOT_RESERVED);
+                continue;
+            }
+            const int64_t dst = layer0 + (((int64_t)page[n] << shift) + (at & (c.page_size - 1))) * row + h * c.head_dim + d;
+            *(u32x4v *)((uint16_t *)c.k_pages + dst) = x[n];
+            *(u32x4v *)((uint16_t *)c.v_pages + dst) = y[n];
+        }
     }
 }
 
@@ -333,7 +348,7 @@ __device__ int keep_ok(const FaCache &c, const int32_t *slots, int n, int i, con
 
 // Moves the kept rows together, in place. A lane owns 16 bytes of a row in one layer of K or V and moves them in
 // ascending order: a row's new place is at or before its old one and before every later row's, so nothing is
-// overwritten before it is read; eight rows are read before the first of them is written.
+// overwritten before it is read; sixteen rows are read before the first of them is written.
 __global__ __launch_bounds__(128) void cache_move_kernel(const FaCache c, const int32_t *slots, int n,
                                                          const int32_t *keep, int64_t keep_stride, int max_keep,
                                                          const int32_t *counts) {
@@ -348,13 +363,13 @@ __global__ __launch_bounds__(128) void cache_move_kernel(const FaCache c, const 
     const int64_t row = (int64_t)c.nheads * c.head_dim;
     uint16_t *pool = (uint16_t *)(blockIdx.y & 1 ? c.v_pages : c.k_pages) +
                      (int64_t)(blockIdx.y >> 1) * c.num_pages * c.page_size * row + ch * 8;
-    for (int j = 0; j < m; j += 8) {
-        u32x4v v[8];
+    for (int j = 0; j < m; j += 16) {
+        u32x4v v[16];
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
+        for (int x = 0; x < 16; ++x)
             if (j + x < m && src[j + x] != dst[j + x]) v[x] = *(const u32x4v *)(pool + src[j + x] * row);
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
+        for (int x = 0; x < 16; ++x)
             if (j + x < m && src[j + x] != dst[j + x]) *(u32x4v *)(pool + dst[j + x] * row) = v[x];
     }
 }
@@ -507,11 +522,10 @@ int fa_cache_write(const FaCache *c, int32_t layer, const int32_t *slots, int32_
     if ((((uintptr_t)k | (uintptr_t)v) & 15) != 0 || (k_rs | k_hs | v_rs | v_hs) % 8)
         return set_error(FA_ERR_INVALID_ARGUMENT, "fa_cache_write: k and v must be 16-byte aligned with strides multiple of 8");
     const int chunks = c->nheads * c->head_dim / 8;
-    int tok = 1024 / chunks;                 // four 16-byte pieces of K and of V to a lane
-    tok = tok < 1 ? 1 : tok;
-    const dim3 grid((max_seqlen + tok - 1) / tok, n);
+    const int lines = chunks < 256 ? 256 / chunks : 1;       // tokens a block takes at a time
+    const dim3 grid((max_seqlen + lines * WRITE_STEPS - 1) / (lines * WRITE_STEPS), n);
     hipLaunchKernelGGL(cache_write_kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, layer, slots, (const uint16_t *)k,
-                       k_rs, k_hs, (const uint16_t *)v, v_rs, v_hs, cu, total, tok);
+                       k_rs, k_hs, (const uint16_t *)v, v_rs, v_hs, cu, total, lines);
     return launched("fa_cache_write");
 }
 

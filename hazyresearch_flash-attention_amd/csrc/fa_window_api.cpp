@@ -149,7 +149,9 @@ int check_paged(const FaPagedArgs *a, const char *fn) {
 
 // Shape and split of a paged call. 32 packed rows or fewer (single tokens, small groups): four waves of a
 // workgroup take the same rows and every fourth tile; up to 64: two and two; more: 128 rows to a workgroup.
-// The split cuts the keys until the workgroups fill the card, with two tiles at least for each wave.
+// (Eight waves on 256 rows, four tiles in flight, took 120 us for 64 drafts over 8 caches of 32000 keys where four waves,
+// two workgroups to a CU, take 102: all eight wait at each barrier.) The keys are split where that makes the rounds of
+// workgroups shorter: steps of a round and 4 more for its start and end, 2 for the join and an eighth for each part.
 struct PagedPlan { WinShape shape; int nrb, nsplit; };
 PagedPlan plan_paged(const FaPagedArgs *a) {
     PagedPlan p;
@@ -168,10 +170,18 @@ PagedPlan plan_paged(const FaPagedArgs *a) {
     const int64_t base = (int64_t)p.nrb * a->nheads_k * a->batch;
     int cus = device_cus();
     if (cus <= 0) cus = 256;
-    int64_t want = (2 * cus + base - 1) / base;
-    const int64_t most = tiles / (2 * kg);
-    want = want < most ? want : most;
-    want = want < 1 ? 1 : (want > 128 ? 128 : want);
+    // workgroups that a CU holds at once (LDS and registers of the shapes, by head-dim tile)
+    const int per_cu = (p.shape == WIN_1X4X32 ? 1 : 2) * (tile_of(a->head_dim) == 128 ? 1 : 2);
+    const int64_t slots = (int64_t)cus * per_cu;
+    int64_t want = 1, best = 0;
+    for (int64_t n = 1; n <= 128 && (n == 1 || 2 * kg * n <= tiles); ++n) {
+        const int64_t rounds = (base * n + slots - 1) / slots, steps = ((tiles + n - 1) / n + kg - 1) / kg;
+        const int64_t cost = rounds * (steps + 4) + (n > 1 ? 2 : 0) + n / 8;
+        if (n == 1 || cost < best) {
+            best = cost;
+            want = n;
+        }
+    }
     p.nsplit = (int)want;
     return p;
 }

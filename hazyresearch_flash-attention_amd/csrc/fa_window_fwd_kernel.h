@@ -171,20 +171,24 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         const int p = wr + NWR * i;
         const int r = C::RPP * p + lane / C::NC;
         const int c = (lane % C::NC) ^ S::x(r);
-        const int rr = PAGED ? lane / C::NC : r;              // paged: each piece has a base of its own
         const bool ok = c * 8 < head_dim;
-        k_off[i] = ok ? (rr * (int)a.k_rs + c * 8) * 2 : OOB;
-        v_off[i] = ok ? (rr * (int)a.v_rs + c * 8) * 2 : OOB;
+        k_off[i] = ok ? (r * (int)a.k_rs + c * 8) * 2 : OOB;
+        v_off[i] = ok ? (r * (int)a.v_rs + c * 8) * 2 : OOB;
     }
     constexpr int NU = BN / 16;                               // a page holds 16 rows or more
+    const bool one_page = PAGED && (1 << a.page_shift) >= BN; // pages of whole tiles: one entry to a tile
     int ent[NU];                                              // table entries of the tile to be staged next
     auto load_entries = [&](int i) __attribute__((always_inline)) {
         if constexpr (PAGED) {
             const int j0 = walk.tile(i) * BN;
+            const int last = a.max_blocks - 1, b0 = j0 >> a.page_shift;
+            ent[0] = uniform_load(tbl + (b0 < last ? b0 : last));
+            if (!one_page) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const int blk = (j0 + 16 * u) >> a.page_shift;
-                ent[u] = uniform_load(tbl + (blk < a.max_blocks ? blk : a.max_blocks - 1));
+                for (int u = 1; u < NU; ++u) {
+                    const int blk = (j0 + 16 * u) >> a.page_shift;
+                    ent[u] = uniform_load(tbl + (blk < last ? blk : last));
+                }
             }
         }
     };
@@ -194,23 +198,43 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         char *kb = gsm + buf * C::TILE, *vb = gsm + (2 + buf) * C::TILE;
         uint32_t there = 0;
         if constexpr (PAGED) {
+            // rows of a page from row `rin` on stand at the tile's rows from `r0` on; what is not there is not read
+            auto rows_of = [&](int e, int r0, int n, i32x4 &ks, i32x4 &vs) __attribute__((always_inline)) {
+                const bool ok = (uint32_t)e < (uint32_t)a.num_pages;
+                int rows = klen - (j0 + r0);
+                rows = !ok || rows < 0 ? 0 : (rows > n ? n : rows);
+                const int64_t pg = ok ? e : 0, rin = ((j0 + r0) & ((1 << a.page_shift) - 1)) - r0;
+                const int end = rows > 0 ? r0 + rows : 0;
+                ks = make_srd(kbase + pg * a.k_ps + rin * a.k_rs, end * (int)a.k_rs * 2);
+                vs = make_srd(vbase + pg * a.v_ps + rin * a.v_rs, end * (int)a.v_rs * 2);
+            };
+            i32x4 ks, vs;
+            if (one_page) {
+                there = (uint32_t)ent[0] < (uint32_t)a.num_pages ? (1u << NU) - 1 : 0u;
+                rows_of(ent[0], 0, BN, ks, vs);
 #pragma unroll
-            for (int u = 0; u < NU; ++u) there |= ((uint32_t)ent[u] < (uint32_t)a.num_pages ? 1u : 0u) << u;
+                for (int n = 0; n < C::PPW; ++n) {
+                    const int p = wr + NWR * n;
+                    if (C::PIECES % NWR == 0 || p < C::PIECES) {
+                        dma16(ks, k_off[n], 0, lds_addr(kb + 1024 * p));
+                        dma16(vs, v_off[n], 0, lds_addr(vb + 1024 * p));
+                    }
+                }
+            } else {
 #pragma unroll
-            for (int n = 0; n < C::PPW; ++n) {
-                const int p = wr + NWR * n;
-                if (C::PIECES % NWR == 0 || p < C::PIECES) {
-                    const int j = j0 + C::RPP * p;
-                    const int u = C::RPP * p / 16;
-                    int e = ent[0];
+                for (int u = 0; u < NU; ++u) there |= ((uint32_t)ent[u] < (uint32_t)a.num_pages ? 1u : 0u) << u;
 #pragma unroll
-                    for (int x = 1; x < NU; ++x) e = u == x ? ent[x] : e;
-                    const bool ok = (uint32_t)e < (uint32_t)a.num_pages;
-                    int rows = klen - j;
-                    rows = !ok || rows < 0 ? 0 : (rows > C::RPP ? C::RPP : rows);
-                    const int64_t pg = ok ? e : 0, rin = j & ((1 << a.page_shift) - 1);
-                    dma16(make_srd(kbase + pg * a.k_ps + rin * a.k_rs, rows * (int)a.k_rs * 2), k_off[n], 0, lds_addr(kb + 1024 * p));
-                    dma16(make_srd(vbase + pg * a.v_ps + rin * a.v_rs, rows * (int)a.v_rs * 2), v_off[n], 0, lds_addr(vb + 1024 * p));
+                for (int n = 0; n < C::PPW; ++n) {
+                    const int p = wr + NWR * n;
+                    if (C::PIECES % NWR == 0 || p < C::PIECES) {
+                        const int u = C::RPP * p / 16;
+                        int e = 0;             // ent[u], u the wave's: by masks (an index would put ent in memory)
+#pragma unroll
+                        for (int x = 0; x < NU; ++x) e |= ent[x] & -(int)(u == x);
+                        rows_of(e, C::RPP * p, C::RPP, ks, vs);
+                        dma16(ks, k_off[n], 0, lds_addr(kb + 1024 * p));
+                        dma16(vs, v_off[n], 0, lds_addr(vb + 1024 * p));
+                    }
                 }
             }
         } else {
@@ -233,10 +257,10 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
 
     // ---- the first tile is on its way before the rows are read
     auto idx = [&](int n) __attribute__((always_inline)) -> int { return i_beg + KG * n + kg; };
-    uint32_t there = 0, there_n = 0;
+    uint32_t there[2] = {0, 0};
     if (idx(0) < i_end) {
         load_entries(idx(0));
-        there = stage(idx(0), 0);
+        there[0] = stage(idx(0), 0);
     }
     if (idx(1) < i_end) load_entries(idx(1));
 
@@ -399,8 +423,9 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
                 }
     };
 
-    // ---- the walk: stage tile n+1, compute tile n, wait, meet
-    auto meet = [&]() __attribute__((always_inline)) {
+    // ---- the walk: wait for tile n, meet, stage tile n + 1 (over tile n - 1, which all have read), compute tile n
+    auto step = [&](auto par, int n) __attribute__((always_inline)) {
+        constexpr int P = decltype(par)::value;
         vmcnt0();
         if constexpr (NWR > 1) {
             __syncthreads();
@@ -409,20 +434,14 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
             __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
             asm volatile("" ::: "memory");
         }
-    };
-    if (steps > 0) meet();
-    auto step = [&](auto par, int n) __attribute__((always_inline)) {
-        constexpr int P = decltype(par)::value;
-        const int i = idx(n);
-        if (idx(n + 1) < i_end) there_n = stage(idx(n + 1), 1 - P);
+        if (idx(n + 1) < i_end) there[1 - P] = stage(idx(n + 1), 1 - P);
         if (idx(n + 2) < i_end) load_entries(idx(n + 2));
+        const int i = idx(n);
         if (i < i_end) {
             const int j0 = walk.tile(i) * BN;
             // a tile that none of the wave's rows sees adds nothing
-            if (rw < R && j0 <= pmax && (j0 + BN - 1 > pmin - a.window || j0 < a.sinks)) compute(j0, P, there);
+            if (rw < R && j0 <= pmax && (j0 + BN - 1 > pmin - a.window || j0 < a.sinks)) compute(j0, P, there[P]);
         }
-        there = there_n;
-        meet();
     };
     for (int n = 0; n < steps; n += 2) {
         step(std::integral_constant<int, 0>(), n);
@@ -550,6 +569,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     const bool empty = mrow == -INFINITY && l_tot == 0.f;
     const float inv = empty ? 0.f : 1.f / l_tot;
     if constexpr (KG == 1) {
+        __syncthreads();
         store_rows<D, T>(o, inv, smem + wave * 64 * D, head_dim, [&](int r) __attribute__((always_inline)) -> uint16_t * {
             if (rw + r >= R) return nullptr;
             const int tt = a.dgroup.div(rw + r), gg = rw + r - tt * G;
@@ -577,8 +597,9 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         a.lse[(int64_t)(b * a.nheads + kvh * G + g) * a.lse_stride + t] = empty ? -INFINITY : mrow * LN2 + __logf(l_tot);
 }
 
-// Joins the splits of a row: O = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - max m), in the splits' order.
-// One wave to a row; bound by launch and by reading the partials once.
+// Joins the splits of a row: O = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - max m), in a fixed order. One wave to
+// a row: its lanes take the splits' m and l (two each, 128 splits at most), then the columns, eight splits' loads in
+// flight. Bound by launch and two loads one after the other (5.9 us with a loop of single loads, 8 splits).
 template <int D, typename T>
 __global__ __launch_bounds__(256) void fa_window_join_kernel(const WinFwdArgs a) {
     constexpr float LN2 = 0.6931471805599453f;
@@ -589,28 +610,47 @@ __global__ __launch_bounds__(256) void fa_window_join_kernel(const WinFwdArgs a)
     const int lane = threadIdx.x & 63;
     if (i >= (int64_t)sq * a.nheads) return;
     const int64_t row = (int64_t)q_start * a.nheads + i, rows = a.total_q * a.nheads;
-    float top = -INFINITY;
-    for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, a.ws_ml[(s * rows + row) * 2]);
     constexpr int E = D >= 64 ? D / 64 : 1;
-    float acc[E], l = 0.f;
+    typedef float vec __attribute__((ext_vector_type(E)));
+    float m[2], w[2], top = -INFINITY, l = 0.f;
+    float ls[2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float m = a.ws_ml[(s * rows + row) * 2], ls = a.ws_ml[(s * rows + row) * 2 + 1];
-        const float w = m == -INFINITY ? 0.f : fast_exp2(m - top);
-        l += w * ls;
-        const float *op = a.ws_o + (s * rows + row) * D;
+    for (int x = 0; x < 2; ++x) {
+        const int s = lane + 64 * x;
+        m[x] = s < a.nsplit ? a.ws_ml[(s * rows + row) * 2] : -INFINITY;
+        ls[x] = s < a.nsplit ? a.ws_ml[(s * rows + row) * 2 + 1] : 0.f;
+        top = fmaxf(top, m[x]);
+    }
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (D >= 64 || lane < D) acc[e] += w * op[E * lane + e];
+    for (int s = 32; s >= 1; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        w[x] = m[x] == -INFINITY ? 0.f : fast_exp2(m[x] - top);
+        l += m[x] == -INFINITY ? ls[x] * 0.f : w[x] * ls[x];       // (a NaN stays one)
+    }
+    l = wave_sum(l);
+    const int e0 = D >= 64 || lane < D ? E * lane : 0;
+    const float *op = a.ws_o + row * D + e0;
+    vec acc = {};
+    for (int s0 = 0; s0 < a.nsplit; s0 += 8) {
+        vec v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (s0 + x < a.nsplit) v[x] = *(const vec *)(op + (s0 + x) * rows * D);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (s0 + x < a.nsplit) acc += v[x] * __shfl(s0 < 64 ? w[0] : w[1], (s0 + x) & 63);
     }
     const bool empty = top == -INFINITY && l == 0.f;
     const float inv = empty ? 0.f : 1.f / l;
     const int t = (int)(i / a.nheads), h = (int)(i - (int64_t)t * a.nheads);
-    uint16_t *op = a.o + (int64_t)(q_start + t) * a.o_rs + (int64_t)h * a.o_hs;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (E * lane + e < a.head_dim) op[E * lane + e] = T::from_float(acc[e] * inv);
+    uint16_t *out = a.o + (int64_t)(q_start + t) * a.o_rs + (int64_t)h * a.o_hs + e0;
+    if (e0 < a.head_dim && (D >= 64 || lane < D)) {
+        if constexpr (E == 2)
+            *(uint32_t *)out = T::pack2(acc[0] * inv, acc[1] * inv);
+        else
+            *out = T::from_float(acc[0] * inv);
+    }
     if (lane == 0 && a.lse)
         a.lse[(int64_t)(b * a.nheads + h) * a.lse_stride + t] = empty ? -INFINITY : top * LN2 + __logf(l);
 }

@@ -7,7 +7,7 @@ namespace fa {
 struct WinFwdArgs;
 struct WinBwdArgs;
 // `shape` of a forward launch: row waves x key groups x keys per tile
-enum WinShape { WIN_4X1X64 = 0, WIN_2X2X32 = 1, WIN_1X4X32 = 2 };
+enum WinShape { WIN_4X1X64, WIN_2X2X32, WIN_1X4X32 };
 int win_shape_rows(WinShape s);      // packed rows per workgroup
 int win_shape_groups(WinShape s);
 int win_shape_keys(WinShape s);      // keys per tile
