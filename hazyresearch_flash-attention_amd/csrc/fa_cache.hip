@@ -131,7 +131,8 @@ __global__ __launch_bounds__(1024) void cache_reserve_kernel(const FaCache c, co
         return;
     }
     // a shared page is copied unless this is its last holder: earlier slots of the call leave it first
-    long long mine = 0;                                  // pages needed, and copies above them
+    long long mine = 0;                                  // pages needed (4096 times 2^26 at most), copies above them
+    constexpr int COPY_BIT = 48;
     int need[RES_PER];
     bool copy[RES_PER];
 #pragma unroll
@@ -152,12 +153,18 @@ __global__ __launch_bounds__(1024) void cache_reserve_kernel(const FaCache c, co
         }
         const int more = blocks_of((int64_t)len[x] + cnt[x], ps) - have[x];
         need[x] = (copy[x] ? 1 : 0) + (more > 0 ? more : 0);
-        mine += need[x] + ((long long)copy[x] << 32);
+        mine += need[x] + ((long long)copy[x] << COPY_BIT);
     }
     long long sums;
     const long long at0 = scan1024<long long>(mine, tmp[0], sums);
-    const int total = (int)sums, ncopies = (int)(sums >> 32);
-    if (total == 0) return;
+    const int ncopies = (int)(sums >> COPY_BIT);
+    const long long wanted = sums & ((1ll << COPY_BIT) - 1);
+    if (wanted == 0) return;
+    if (wanted > c.num_pages) {
+        if (tid == 0) flag(c, FA_CACHE_NO_PAGES);
+        return;
+    }
+    const int total = (int)wanted;
     // the `total` lowest free pages, in order
     int32_t *list = c.scratch + SCR_FREE;
     int found = 0;
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(1024) void cache_reserve_kernel(const FaCache c, co
     __syncthreads();
     // the tables: a thread sets its slots' copies and first new blocks, its wave the rest of long ones
     constexpr int OWN = 4;
-    int rank = (int)at0, crank = (int)(at0 >> 32);
+    int rank = (int)(at0 & ((1ll << COPY_BIT) - 1)), crank = (int)(at0 >> COPY_BIT);
 #pragma unroll
     for (int x = 0; x < RES_PER; ++x) {
         const int64_t row = (int64_t)slot[x] * c.max_blocks;
@@ -261,14 +268,10 @@ constexpr int WRITE_STEPS = 4;
 __global__ __launch_bounds__(256) void cache_write_kernel(const FaCache c, int layer, const int32_t *slots,
                                                           const uint16_t *k, int64_t k_rs, int64_t k_hs,
                                                           const uint16_t *v, int64_t v_rs, int64_t v_hs,
-                                                          const int32_t *cu, int64_t total, int lines) {
+                                                          const int32_t *cu, int64_t total, int n, int lines) {
     const int i = blockIdx.y, s = slots[i];
     int beg = cu[i], end = cu[i + 1];
-    if (s == -1) return;
-    if (s < 0 || s >= c.max_seqs) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) flag(c, FA_CACHE_BAD_SLOT);
-        return;
-    }
+    if (s == -1 || !slot_ok(c, slots, n, i, s)) return;
     beg = beg < 0 ? 0 : beg;
     end = end > total ? (int)total : end;
     const int hc = c.head_dim / 8, chunks = c.nheads * hc;
@@ -525,7 +528,7 @@ int fa_cache_write(const FaCache *c, int32_t layer, const int32_t *slots, int32_
     const int lines = chunks < 256 ? 256 / chunks : 1;       // tokens a block takes at a time
     const dim3 grid((max_seqlen + lines * WRITE_STEPS - 1) / (lines * WRITE_STEPS), n);
     hipLaunchKernelGGL(cache_write_kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, layer, slots, (const uint16_t *)k,
-                       k_rs, k_hs, (const uint16_t *)v, v_rs, v_hs, cu, total, lines);
+                       k_rs, k_hs, (const uint16_t *)v, v_rs, v_hs, cu, total, n, lines);
     return launched("fa_cache_write");
 }
 

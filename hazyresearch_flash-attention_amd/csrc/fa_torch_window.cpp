@@ -36,7 +36,7 @@ at::Tensor rows(const at::Tensor &t) {
 
 void check_i32(const at::Tensor &t, const char *name, const at::Tensor &like) {
     TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32");
-    TORCH_CHECK(t.device() == like.device(), name, " must be on the device of q");
+    TORCH_CHECK(t.device() == like.device(), name, " must be on the device ", like.device());
 }
 
 void check_cu(const at::Tensor &t, const char *name, const at::Tensor &like) {
@@ -385,7 +385,7 @@ struct Cache {
         : k(k_), v(v_), table(table_), seqlens(seqlens_), nblocks(nblocks_), refcount(refcount_), status(status_) {
         TORCH_CHECK(k.is_cuda(), "the cache must be on the GPU");
         dtype_of(k);
-        TORCH_CHECK(k.dim() == 5 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.dtype() == k.dtype(),
+        TORCH_CHECK(k.dim() == 5 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes() && v.dtype() == k.dtype() && v.device() == k.device(),
                     "k, v must be (layers, num_pages, page_size, nheads, headdim), contiguous");
         for (const at::Tensor *t : {&table, &seqlens, &nblocks, &refcount, &status}) {
             check_i32(*t, "the cache's tables", k);

@@ -72,7 +72,8 @@ int check_window(const FaWindowArgs *a, const char *fn, bool bwd) {
     if (a->reserved != 0) return set_error(FA_ERR_INVALID_ARGUMENT, "%s: reserved must be 0", fn);
     if (a->max_seqlen_k < 0 || a->total_q < 0 || a->total_k < 0)
         return set_error(FA_ERR_INVALID_ARGUMENT, "%s: negative length", fn);
-    if ((a->total_q + a->total_k + a->max_seqlen_q) * (a->nheads / a->nheads_k) >= LEN_LIMIT || a->max_seqlen_k >= LEN_LIMIT)
+    if (a->total_q >= LEN_LIMIT || a->total_k >= LEN_LIMIT || a->max_seqlen_k >= LEN_LIMIT ||
+        (a->total_q + a->total_k + a->max_seqlen_q) * (a->nheads / a->nheads_k) >= LEN_LIMIT)
         return set_error(FA_ERR_UNSUPPORTED, "%s: 2^30 or more rows", fn);
     if (!a->cu_seqlens_q || !a->cu_seqlens_k) return set_error(FA_ERR_INVALID_ARGUMENT, "%s: cu_seqlens is NULL", fn);
     if (a->lse_stride < a->max_seqlen_q) return set_error(FA_ERR_INVALID_ARGUMENT, "%s: lse_stride < max_seqlen_q", fn);
@@ -116,7 +117,7 @@ int check_paged(const FaPagedArgs *a, const char *fn) {
         return set_error(FA_ERR_UNSUPPORTED, "%s: page_size must be a power of two, 16 or more (got %d)", fn, a->page_size);
     if (a->num_pages < 0 || a->num_seqs < 0 || a->max_blocks < 0)
         return set_error(FA_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
-    if ((int64_t)a->max_blocks * a->page_size >= LEN_LIMIT ||
+    if ((int64_t)a->max_blocks * a->page_size >= LEN_LIMIT || a->total_q >= LEN_LIMIT ||
         (a->total_q + a->max_seqlen_q) * (a->nheads / a->nheads_k) >= LEN_LIMIT)
         return set_error(FA_ERR_UNSUPPORTED, "%s: 2^30 or more rows or keys", fn);
     if (a->tree_mask && (a->tree_words < 1 || a->tree_words > 4 || a->max_seqlen_q > 64 * a->tree_words))
@@ -255,6 +256,7 @@ int fa_window_fwd(const FaWindowArgs *a, void *stream) {
     w.total_q = a->total_q; w.total_k = a->total_k;
     w.batch = a->batch; w.nheads = a->nheads; w.nheads_k = a->nheads_k; w.head_dim = a->head_dim;
     w.group = a->nheads / a->nheads_k;
+    w.max_q = a->max_seqlen_q;
     w.lse_stride = a->lse_stride;
     w.window = a->window > 0 && a->window < NO_WINDOW ? a->window : NO_WINDOW;
     w.sinks = a->num_sinks;
@@ -282,7 +284,7 @@ int64_t fa_window_bwd_workspace(const FaWindowArgs *a) {
     const int rc = check_sizes("fa_window_bwd_workspace", a->batch, a->nheads, a->nheads_k, a->head_dim, a->max_seqlen_q,
                                a->window, a->num_sinks, a->softmax_scale, a->dtype);
     if (rc) return -rc;
-    if (a->total_q < 0 || a->total_k < 0 || a->max_seqlen_k < 0 ||
+    if (a->total_q < 0 || a->total_k < 0 || a->max_seqlen_k < 0 || a->total_q >= LEN_LIMIT || a->total_k >= LEN_LIMIT ||
         (a->total_q + a->total_k + a->max_seqlen_q) * (a->nheads / a->nheads_k) >= LEN_LIMIT)
         return -set_error(FA_ERR_INVALID_ARGUMENT, "fa_window_bwd_workspace: lengths out of range");
     WinBwdArgs w{};
@@ -310,6 +312,7 @@ int fa_window_bwd(const FaWindowArgs *a, void *stream) {
     w.group = a->nheads / a->nheads_k;
     w.dgroup = Div::of(w.group);
     w.dheads = Div::of(w.nheads_k);
+    w.max_q = a->max_seqlen_q;
     w.lse_stride = a->lse_stride;
     w.scale = a->softmax_scale;
     int64_t bytes;
@@ -360,7 +363,7 @@ int fa_paged_fwd(const FaPagedArgs *a, void *stream) {
     w.group = a->nheads / a->nheads_k;
     w.num_pages = a->num_pages; w.num_seqs = a->num_seqs; w.max_blocks = a->max_blocks;
     w.page_shift = __builtin_ctz(a->page_size);
-    w.tree_words = a->tree_words; w.lse_stride = a->lse_stride;
+    w.tree_words = a->tree_words; w.max_q = a->max_seqlen_q; w.lse_stride = a->lse_stride;
     w.window = a->window > 0 && a->window < NO_WINDOW ? a->window : NO_WINDOW;
     w.sinks = a->num_sinks;
     w.nrb = p.nrb; w.nsplit = p.nsplit;

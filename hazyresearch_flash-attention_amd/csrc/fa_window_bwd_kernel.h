@@ -30,7 +30,7 @@ struct WinBwdArgs {
     int64_t dq_rs, dq_hs, dk_rs, dk_hs, dv_rs, dv_hs;
     int64_t total_q, total_k;
     int batch, nheads, nheads_k, head_dim, group;
-    int lse_stride, window, sinks;
+    int max_q, lse_stride, window, sinks;
     // the sinks' rows behind the window, cut into `chunks` shares (0: walked with the rest): blocks of 32 keys,
     // partial sums a share leaves (one for each wave or pair), `slots` of them in all and the window's own
     int chunks, sink_blocks, per_chunk, slots;
@@ -40,8 +40,8 @@ struct WinBwdArgs {
 };
 
 // first packed row (of the whole tensor's row constants) of a sequence and key/value head
-__device__ __forceinline__ int64_t rows_base(const WinBwdArgs &a, int q_start, int sq, int kvh) {
-    return (int64_t)q_start * a.nheads + (int64_t)kvh * sq * a.group;
+__device__ __forceinline__ int64_t rows_base(const WinBwdArgs &a, int q_start, int len_q, int kvh) {
+    return (int64_t)q_start * a.nheads + (int64_t)kvh * len_q * a.group;
 }
 
 // ---------------------------------------------------------------------------------------------- dQ
@@ -77,10 +77,10 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
     a.order.get(blockIdx.x, rb, w);
     const int b = a.dheads.div(w);
     const int kvh = w - b * a.nheads_k;
-    int q_start, sq, k_start, klen;
-    seq_bounds(a.cu_q, b, a.total_q, q_start, sq);
+    int q_start, len_q, k_start, klen;
+    seq_bounds(a.cu_q, b, a.total_q, q_start, len_q);
     seq_bounds(a.cu_k, b, a.total_k, k_start, klen);
-    const int off = klen - sq;
+    const int off = klen - len_q, sq = len_q < a.max_q ? len_q : a.max_q;     // lse's rows end at max_q
     const int G = a.group, R = sq * G, r0 = rb * C::BM;
     if (r0 >= R) {
         zero_tail(a.dq, a.dq_rs, a.dq_hs, a.nheads, a.head_dim, a.total_q, a.cu_q, a.batch);
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
         delta = pair_sum(dsum);
         if (walk.n > 0) stage(0, 0);
     }
-    if (hi == 0 && row < R) a.ws_rows[rows_base(a, q_start, sq, kvh) + row] = f32x2{lse2, -delta};
+    if (hi == 0 && row < R) a.ws_rows[rows_base(a, q_start, len_q, kvh) + row] = f32x2{lse2, -delta};
     walk_all(std::false_type{});
 
     // an infinity or NaN: this wave's rows again, key by key (fa_window_careful.h)
@@ -359,10 +359,10 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
     }
     const int b = a.dheads.div(w);
     const int kvh = w - b * a.nheads_k;
-    int q_start, sq, k_start, klen;
-    seq_bounds(a.cu_q, b, a.total_q, q_start, sq);
+    int q_start, len_q, k_start, klen;
+    seq_bounds(a.cu_q, b, a.total_q, q_start, len_q);
     seq_bounds(a.cu_k, b, a.total_k, k_start, klen);
-    const int off = klen - sq;
+    const int off = klen - len_q, sq = len_q < a.max_q ? len_q : a.max_q;     // lse's rows end at max_q
     const int G = a.group, k0 = kb * (sink ? 32 : C::BK);
     if (k0 >= klen) {              // (a sink that is not there leaves no sums: its dK, dV have no row)
         tails();
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
     // ---- staging of tile n: row r is token r / G of head kvh G + r % G; rows behind the last land as zeros
     const uint16_t *qbase = a.q + (int64_t)q_start * a.q_rs + (int64_t)kvh * G * a.q_hs;
     const uint16_t *dbase = a.dout + (int64_t)q_start * a.do_rs + (int64_t)kvh * G * a.do_hs;
-    const f32x2 *rows_g = a.ws_rows + rows_base(a, q_start, sq, kvh);
+    const f32x2 *rows_g = a.ws_rows + rows_base(a, q_start, len_q, kvh);
     int q_off[C::PPW], do_off[C::PPW];                 // from the tile's first token
     auto lane_offsets = [&](int rt, int t0, int rows) __attribute__((always_inline)) {
 #pragma unroll

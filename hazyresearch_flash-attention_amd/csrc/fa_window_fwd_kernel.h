@@ -31,7 +31,7 @@ struct WinFwdArgs {
     int64_t table_stride, total_q, total_k;
     int batch, nheads, nheads_k, head_dim, group;
     int num_pages, page_shift, num_seqs, max_blocks, tree_words;
-    int lse_stride, window, sinks, nrb, nsplit;
+    int max_q, lse_stride, window, sinks, nrb, nsplit;
     float scale;
     Div dgroup, dheads, dsplit;   // by group, nheads_k, nsplit
     BlockOrder order;             // dense; paged: its blk divides by nrb
@@ -86,11 +86,11 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     const int b = a.dheads.div(w);
     const int kvh = w - b * a.nheads_k;
 
-    int q_start, sq, klen, off;
+    int q_start, len_q, klen, off;
     const uint16_t *kbase, *vbase;
     const int32_t *tbl = nullptr;
-    seq_bounds(a.cu_q, b, a.total_q, q_start, sq);
-    if (TREE && sq > 64 * a.tree_words) sq = 64 * a.tree_words;   // the masks' rows (and depth_s) end there
+    seq_bounds(a.cu_q, b, a.total_q, q_start, len_q);
+    const int sq = len_q < a.max_q ? len_q : a.max_q;             // lse's rows (masks, depth_s) end at max_q
     const int G = a.group;
     const int R = sq * G;
     const int r0 = rb * C::BM;
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
         const int64_t room = (int64_t)a.max_blocks << a.page_shift;
         if (ctx > room) ctx = (int)room;
         off = ctx;
-        const int64_t end = (int64_t)ctx + sq;
+        const int64_t end = (int64_t)ctx + len_q;
         klen = used ? (int)(end < room ? end : room) : 0;
         tbl = a.table + (int64_t)(used ? row : 0) * a.table_stride;
         kbase = a.k + (int64_t)kvh * a.k_hs;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
     } else {
         int k_start;
         seq_bounds(a.cu_k, b, a.total_k, k_start, klen);
-        off = klen - sq;
+        off = klen - len_q;
         kbase = a.k + (int64_t)k_start * a.k_rs + (int64_t)kvh * a.k_hs;
         vbase = a.v + (int64_t)k_start * a.v_rs + (int64_t)kvh * a.v_hs;
     }
@@ -606,6 +606,7 @@ __global__ __launch_bounds__(256) void fa_window_join_kernel(const WinFwdArgs a)
     int q_start, sq;
     const int b = blockIdx.y;
     seq_bounds(a.cu_q, b, a.total_q, q_start, sq);
+    sq = sq < a.max_q ? sq : a.max_q;
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (i >= (int64_t)sq * a.nheads) return;

@@ -23,7 +23,7 @@ def pack_tree_mask(mask):
         raise RuntimeError(f"a tree holds at most 256 tokens, got {n}")
     words = max(1, (n + 63) // 64)
     m = torch.zeros((rows, words * 64), dtype=torch.int64, device=mask.device)
-    m[:, :n] = mask.to(torch.int64)
+    m[:, :n] = (mask != 0).to(torch.int64)
     shift = torch.arange(64, dtype=torch.int64, device=mask.device)
     return (m.view(rows, words, 64) << shift).sum(-1)     # each bit once: the sum is their union
 

@@ -46,7 +46,8 @@ typedef struct FaWindowArgs {
     int64_t dv_row_stride, dv_head_stride;
     int64_t total_q, total_k;
     int32_t batch, nheads, nheads_k, head_dim;   /* head_dim: multiple of 8, <= 128 */
-    int32_t max_seqlen_q, max_seqlen_k, lse_stride;
+    int32_t max_seqlen_q, max_seqlen_k, lse_stride;   /* rows of a sequence past max_seqlen_q (dk, dv: keys past
+                                     max_seqlen_k) are not computed and not written */
     int32_t window;               /* keys a query sees counting its own position; 0: all */
     int32_t num_sinks;            /* first keys that every later query sees */
     float softmax_scale;
@@ -89,7 +90,8 @@ typedef struct FaPagedArgs {
     int32_t batch, nheads, nheads_k, head_dim;
     int32_t num_pages, page_size; /* page_size: a power of two, 16 or more */
     int32_t num_seqs, max_blocks;
-    int32_t max_seqlen_q, max_context_len;   /* max_context_len: a bound that splits the work; results do not depend on it */
+    int32_t max_seqlen_q, max_context_len;   /* max_seqlen_q as above. max_context_len only decides how the keys are
+                                     split: results differ in the order of their sums, in the last bits */
     int32_t tree_words, lse_stride;
     int32_t window, num_sinks;
     float softmax_scale;

@@ -149,12 +149,7 @@ class Model:
         return (p, j % self.ps) if p >= 0 and self.ref[p] == 1 else None
 
     def write(self, layer, slots, k, v, cu):
-        for i, s in enumerate(slots):
-            if s == -1:
-                continue
-            if not 0 <= s < self.S:
-                self.status |= 4
-                continue
+        for i, s in self.slots_ok(slots):
             for t in range(cu[i], cu[i + 1]):
                 at = self.own(s, self.len[s] + t - cu[i])
                 if at is None:
@@ -370,6 +365,37 @@ def test_offsets_past_32_bits():
         for p in pages:
             for layer in range(L):
                 assert torch.equal(cache.k[layer, p, :12], (k + layer)[rows]) and torch.equal(cache.v[layer, p, :12], (v - layer)[rows])
+
+
+@pytest.mark.gpu
+def test_a_write_names_a_slot_once():
+    c = _cache(2, 8, 16, 2, 64, 3, 2)
+    m = Model(c)
+    c.reserve(_i32([0, 1, 2]), 20)
+    m.reserve([0, 1, 2], [20] * 3)
+    k, v = (torch.randn(60, 2, 64, device="cuda").bfloat16() for _ in range(2))
+    cu = [0, 20, 40, 60]
+    c.write(1, _i32([2, 0, 2]), k, v, _i32(cu), 20)
+    m.write(1, [2, 0, 2], k, v, cu)
+    m.compare(c)
+    with pytest.raises(RuntimeError, match="twice"):
+        c.check()
+
+
+@pytest.mark.gpu
+def test_a_need_of_2_to_the_32_pages():
+    """65 sequences that ask for 2^32 + 1 pages together, of a cache of 8."""
+    blocks = 2 ** 26 - 1
+    c = _cache(1, 8, 16, 1, 8, 65, blocks)
+    want = [blocks] * 64 + [2 ** 32 + 1 - 64 * blocks]
+    assert sum(want) == 2 ** 32 + 1
+    c.reserve(_i32(list(range(65))), _i32([16 * n for n in want]))
+    assert c.status.item() == 1 and not c.nblocks.any() and not c.refcount.any()
+    assert (c.block_table[:, ::997] == -1).all() and (c.block_table[:, :64] == -1).all()
+    c.status.zero_()
+    c.reserve(_i32([64, 3]), 64)
+    c.check()
+    assert c.block_table[64, :4].tolist() == [0, 1, 2, 3] and c.block_table[3, :4].tolist() == [4, 5, 6, 7]
 
 
 @pytest.mark.gpu

@@ -398,6 +398,52 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("most", [0, 1, 10, 40])
+def test_rows_past_max_seqlen_are_left_alone(d, most):
+    """Sequences longer than max_seqlen_q says (C ABI): what is asked for is right, nothing else is written, the rows
+    that are not computed add nothing to dk and dv."""
+    from window_testutil import DEV, cu, randn
+    L, Args = _abi()
+    H, n, m = 4, [150, 7], [170, 30]
+    q, k, v, dout = (randn(i, (sum(n if i in (0, 3) else m), h, d), torch.bfloat16) for i, h in enumerate((H, 2, 2, H)))
+    full = _func()(q, k, v, cu(n), cu(m), 150, 170, 20, 3, return_lse=True)
+    o, lse = torch.full_like(q, 7), torch.full((2 * H * most + 512,), 7.0, device=DEV)
+    a = _valid(Args)
+    g = {x: torch.full_like(y, 7) for x, y in (("dq", q), ("dk", k), ("dv", v))}
+    c = cu(n), cu(m)
+    for name, t in dict(q=q, k=k, v=v, o=o, dout=dout, softmax_lse=lse, cu_seqlens_q=c[0], cu_seqlens_k=c[1], **g).items():
+        setattr(a, name, t.data_ptr())
+    for name, h in dict(q=H, k=2, v=2, o=H, do=H, dq=H, dk=2, dv=2).items():
+        setattr(a, name + "_row_stride", h * d)
+        setattr(a, name + "_head_stride", d)
+    a.total_q, a.total_k, a.batch, a.nheads, a.nheads_k, a.head_dim = sum(n), sum(m), 2, H, 2, d
+    a.max_seqlen_q, a.max_seqlen_k, a.lse_stride, a.window, a.num_sinks = most, 170, most, 20, 3
+    a.softmax_scale = d ** -0.5
+    a.workspace_bytes = L.fa_window_bwd_workspace(ctypes.byref(a))
+    ws = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=DEV)
+    a.workspace = ws.data_ptr()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert L.fa_window_fwd(ctypes.byref(a), stream) == 0 and L.fa_window_bwd(ctypes.byref(a), stream) == 0
+    torch.cuda.synchronize()
+    kept = torch.zeros(sum(n), dtype=torch.bool, device=DEV)
+    for at, x in ((0, n[0]), (n[0], n[1])):
+        kept[at:at + min(x, most)] = True
+    assert (lse[2 * H * most:] == 7).all() and (o[~kept] == 7).all() and (g["dq"][~kept] == 7).all()
+    assert torch.equal(o[kept], full[0][kept])
+    for b in range(2):
+        rows = min(n[b], most)
+        assert torch.equal(lse[:2 * H * most].view(2, H, most)[b, :, :rows], full[1][b, :, :rows])
+    # the same gradients with the other rows' dout at 0
+    x = [t.clone().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(_func()(*x, *c, 150, 170, 20, 3), x, dout * kept[:, None, None])
+    for name, w in zip(("dk", "dv"), want[1:]):
+        # sums of one set of terms in two orders, each rounded once: a step of bf16 apart at most
+        assert (g[name].double() - w.double()).abs().max() <= 2 ** -7 * w.double().abs().max()
+    assert torch.equal(g["dq"][kept], want[0][kept])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [0, 1])
 def test_nothing_to_do(n):
     from window_testutil import cu
