@@ -261,10 +261,10 @@ __global__ __launch_bounds__(256) void cache_copy_kernel(const FaCache c) {
     }
 }
 
-// New rows into their pages: blockIdx.y the slot; a block takes `lines` tokens at a time (a lane one 16-byte piece of
-// the row, in K and in V), WRITE_STEPS times, all loads before the first store: bound by HBM for long calls, by launch
-// and three dependent loads (length, table, row) for short ones.
-constexpr int WRITE_STEPS = 4;
+// New rows into their pages: blockIdx.y the slot; a block takes `lines` tokens, a lane one 16-byte piece of a row, in K
+// and in V. Bound by HBM for long calls (16 sequences of 8192 tokens, 8 heads of 128: 209 us, 5.1 TB/s; with four tokens
+// to a lane, and a quarter of the blocks, 226), by launch and three dependent loads (length, table, count) for short
+// ones (64 sequences of 25 tokens, 8 heads of 128: 6.1 us against 7.5).
 __global__ __launch_bounds__(256) void cache_write_kernel(const FaCache c, int layer, const int32_t *slots,
                                                           const uint16_t *k, int64_t k_rs, int64_t k_hs,
                                                           const uint16_t *v, int64_t v_rs, int64_t v_hs,
@@ -275,43 +275,27 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const FaCache c, int l
     beg = beg < 0 ? 0 : beg;
     end = end > total ? (int)total : end;
     const int hc = c.head_dim / 8, chunks = c.nheads * hc;
-    const int t0 = beg + blockIdx.x * lines * WRITE_STEPS;
+    const int t0 = beg + blockIdx.x * lines;
     if (t0 >= end) return;
     const int len = c.seqlens[s], have = c.nblocks[s], shift = __builtin_ctz(c.page_size);
     const int64_t row = (int64_t)c.nheads * c.head_dim, layer0 = (int64_t)layer * c.num_pages * c.page_size * row;
-    const int32_t *tbl = c.block_table + (int64_t)s * c.max_blocks;
-    // rows wider than a block: several pieces to a lane, one token at a time
-    for (int ch0 = 0; ch0 < chunks; ch0 += 256) {
-        const int line = lines > 1 ? threadIdx.x / chunks : 0;
-        const int ch = lines > 1 ? threadIdx.x - line * chunks : ch0 + threadIdx.x;
-        if (line >= lines || ch >= chunks) continue;
+    // rows wider than a block: several pieces to a lane
+    const int line = lines > 1 ? threadIdx.x / chunks : 0, t = t0 + line;
+    const int at = len + t - beg, blk = at >> shift;
+    if (line >= lines || t >= end) return;
+    const int page = at >= 0 && blk < have ? c.block_table[(int64_t)s * c.max_blocks + blk] : -1;
+    const bool own = page >= 0 && page < c.num_pages && c.refcount[page] == 1;
+    const int64_t to = layer0 + (((int64_t)page << shift) + (at & (c.page_size - 1))) * row;
+    for (int ch = threadIdx.x - line * chunks; ch < chunks; ch += 256) {
         const int h = ch / hc, d = (ch - h * hc) * 8;
-        const uint16_t *kp = k + (int64_t)h * k_hs + d, *vp = v + (int64_t)h * v_hs + d;
-        u32x4v x[WRITE_STEPS], y[WRITE_STEPS];
-        int page[WRITE_STEPS];
-#pragma unroll
-        for (int n = 0; n < WRITE_STEPS; ++n) {
-            const int t = t0 + n * lines + line, at = len + t - beg, blk = at >> shift;
-            page[n] = -1;
-            if (t < end) {
-                page[n] = at >= 0 && blk < have ? tbl[blk] : -2;
-                x[n] = *(const u32x4v *)(kp + (int64_t)t * k_rs);
-                y[n] = *(const u32x4v *)(vp + (int64_t)t * v_rs);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < WRITE_STEPS; ++n) {
-            const int t = t0 + n * lines + line, at = len + t - beg;
-            if (t >= end) continue;
-            if (page[n] < 0 || page[n] >= c.num_pages || c.refcount[page[n]] != 1) {
-                flag(c, FA_CACHE_NOT_RESERVED);
-                continue;
-            }
-            const int64_t dst = layer0 + (((int64_t)page[n] << shift) + (at & (c.page_size - 1))) * row + h * c.head_dim + d;
-            *(u32x4v *)((uint16_t *)c.k_pages + dst) = x[n];
-            *(u32x4v *)((uint16_t *)c.v_pages + dst) = y[n];
+        const u32x4v x = *(const u32x4v *)(k + (int64_t)t * k_rs + (int64_t)h * k_hs + d);
+        const u32x4v y = *(const u32x4v *)(v + (int64_t)t * v_rs + (int64_t)h * v_hs + d);
+        if (own) {
+            *(u32x4v *)((uint16_t *)c.k_pages + to + ch * 8) = x;
+            *(u32x4v *)((uint16_t *)c.v_pages + to + ch * 8) = y;
         }
     }
+    if (!own) flag(c, FA_CACHE_NOT_RESERVED);
 }
 
 // What compact asks of slots[i]; the same answer in both of its kernels, since the first changes no table. Writes
@@ -526,7 +510,7 @@ int fa_cache_write(const FaCache *c, int32_t layer, const int32_t *slots, int32_
         return set_error(FA_ERR_INVALID_ARGUMENT, "fa_cache_write: k and v must be 16-byte aligned with strides multiple of 8");
     const int chunks = c->nheads * c->head_dim / 8;
     const int lines = chunks < 256 ? 256 / chunks : 1;       // tokens a block takes at a time
-    const dim3 grid((max_seqlen + lines * WRITE_STEPS - 1) / (lines * WRITE_STEPS), n);
+    const dim3 grid((max_seqlen + lines - 1) / lines, n);
     hipLaunchKernelGGL(cache_write_kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, layer, slots, (const uint16_t *)k,
                        k_rs, k_hs, (const uint16_t *)v, v_rs, v_hs, cu, total, n, lines);
     return launched("fa_cache_write");
