@@ -457,7 +457,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
             dma16(ds, do_off[i], 0, lds_addr(buf + C::TILE + 1024 * p));
         }
         // (every wave, the same 256 bytes: a stage is then the same number of loads for each)
-        dma4(make_srd(rows_g + rt, left * 8), lane * 4, lds_addr(buf + 2 * C::TILE));
+        dma4(make_srd(rows_g + rt, left * 8), l32 * 8 + hi * 4, lds_addr(buf + 2 * C::TILE));
     };
 
     constexpr int AHEAD = C::AHEAD;
@@ -502,15 +502,32 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
     // X^T += A^T B over the tile's 32 rows: A rows in LDS (transposed reads), B packed in registers
     auto add_t = [&](f32x16 (&x)[D / 32], int rows, const u32x4 (&bv)[2]) __attribute__((always_inline)) {
         const int at = rows + t_rd;
+        auto get = [&](int sg, int dt) __attribute__((always_inline)) -> u32x4 {
+            const int ro = 16 * sg * S::ROW_BYTES;
+            const u32x2 a0 = lds_read_tr(smem, (at ^ (dt << 6)) + ro);
+            const u32x2 a1 = lds_read_tr(smem, (at ^ (dt << 6) ^ 32) + ro + 8 * S::ROW_BYTES);
+            return u32x4{a0[0], a0[1], a1[0], a1[1]};
+        };
+        // A pair's waves have the registers to read ahead: half of the operands before the first product, the rest
+        // beside it; single waves do not (75 us for 70).
+        u32x4 ahead[PAIR ? D / 32 : 1];
+        if constexpr (PAIR) {
 #pragma unroll
-        for (int sg = 0; sg < 2; ++sg)
+            for (int dt = 0; dt < D / 32; ++dt) ahead[dt] = get(0, dt);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int sg = 0; sg < 2; ++sg) {
 #pragma unroll
             for (int dt = 0; dt < D / 32; ++dt) {
-                const int ro = 16 * sg * S::ROW_BYTES;
-                const u32x2 a0 = lds_read_tr(smem, (at ^ (dt << 6)) + ro);
-                const u32x2 a1 = lds_read_tr(smem, (at ^ (dt << 6) ^ 32) + ro + 8 * S::ROW_BYTES);
-                x[dt] = T::mfma32(as_frag<T>(u32x4{a0[0], a0[1], a1[0], a1[1]}), as_frag<T>(bv[sg]), x[dt]);
+                const u32x4 v = PAIR ? ahead[PAIR ? dt : 0] : get(sg, dt);
+                if constexpr (PAIR)
+                    if (sg == 0) ahead[dt] = get(1, dt);
+                x[dt] = T::mfma32(as_frag<T>(v), as_frag<T>(bv[sg]), x[dt]);
             }
+            if constexpr (PAIR)
+                if (sg == 0) __builtin_amdgcn_sched_barrier(0);
+        }
     };
     auto pack = [&](const f32x16 &x, u32x4 (&out)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -542,19 +559,16 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         const int rt = row_of(n);
         return sink ? n % C::NB == blk : (kw < klen && rt + C::BR > w_lo && rt < w_up);
     };
-    // row constants of registers 4 q4 .. 4 q4 + 3 (rows 8 q4 + 4 hi + e): {lse2, -delta} pairs
-    auto row_consts = [&](int buf, int q4, float (&l)[4], float (&d)[4]) __attribute__((always_inline)) {
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(smem + buf + 2 * C::TILE + (8 * q4 + 4 * hi) * 8);
-        const f32x4 y = *reinterpret_cast<const f32x4 *>(smem + buf + 2 * C::TILE + (8 * q4 + 4 * hi) * 8 + 16);
-        l[0] = x[0]; d[0] = x[1]; l[1] = x[2]; d[1] = x[3];
-        l[2] = y[0]; d[2] = y[1]; l[3] = y[2]; d[3] = y[3];
+    // lse2 (WHICH 0) or -delta (1) of registers 4 q4 .. 4 q4 + 3, rows 8 q4 + 4 hi + e: they lie in LDS one after the
+    // other, not in pairs, so that a read brings nothing that is not used (LDS reads bound this kernel)
+    auto row_const = [&](int which, int buf, int q4) __attribute__((always_inline)) -> f32x4 {
+        return *reinterpret_cast<const f32x4 *>(smem + buf + 2 * C::TILE + (32 * which + 8 * q4 + 4 * hi) * 4);
     };
     auto compute_one = [&](int n, int buf) __attribute__((always_inline)) {
         f32x16 s, dp;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            float l[4], d[4];
-            row_consts(buf, q4, l, d);
+            const f32x4 d = row_const(1, buf, q4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 s[4 * q4 + e] = 0.f;
@@ -570,8 +584,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         }
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            float l[4], d[4];
-            row_consts(buf, q4, l, d);
+            const f32x4 l = row_const(0, buf, q4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fast_exp2(fmaf(s[4 * q4 + e], c_log2, -l[e]));
         }
@@ -600,8 +613,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         char *img = smem + C::OFF_P + (2 * blk + (n & 1)) * 4096;
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            float l[4], d[4];
-            row_consts(buf, q4, l, d);
+            const f32x4 l = row_const(0, buf, q4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fast_exp2(fmaf(s[4 * q4 + e], c_log2, -l[e]));
         }
@@ -618,8 +630,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         read_rows(buf + C::TILE, y);
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-            float l[4], d[4];
-            row_consts(buf, q4, l, d);
+            const f32x4 d = row_const(1, buf, q4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) dp[4 * q4 + e] = d[e];
         }
