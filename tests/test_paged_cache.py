@@ -529,3 +529,59 @@ def test_a_long_generation(graphed):
     c.free(_i32([0, 2, 3]))
     assert not c.refcount.any() and (c.block_table == -1).all()
     c.check()
+
+
+_FIRST_CALL_CAPTURED = """
+import sys
+sys.path[:0] = sys.argv[1:]
+import torch
+from flash_attn.flash_window_attn_interface import flash_window_attn_unpadded_func as window
+from flash_attn.paged_kv_cache import PagedKVCache
+i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+torch.manual_seed(0)
+q, k, v, dout = (torch.randn(300, h, 64, device="cuda").bfloat16().requires_grad_() for h in (4, 2, 2, 4))
+cu = i32([0, 100, 300])
+cache = PagedKVCache(1, 64, 16, 2, 64, 4, 8, window_size=40, num_sinks=2)
+slots, cu2, keep, counts = i32([2, 0]), i32([0, 50, 100]), i32([list(range(50))] * 2), i32([50, 50])
+kn, vn, qn = (torch.randn(100, h, 64, device="cuda").bfloat16() for h in (2, 2, 4))
+
+def step():
+    out = window(q, k, v, cu, cu, 200, 200, 40, 2)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    cache.truncate(slots, i32_zero)
+    cache.reserve(slots, 50)
+    cache.write(0, slots, kn, vn, cu2, 50)
+    o = cache.attend(0, qn, slots, cu2, 50)
+    cache.compact(slots, keep, counts)
+    cache.evict(slots)
+    return [out.detach(), *grads, o, cache.block_table.clone(), cache.seqlens.clone(), cache.refcount.clone()]
+
+i32_zero = i32([0, 0])
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+replays = []
+for _ in range(3):
+    graph.replay()
+    replays.append([x.clone() for x in got])
+    torch.cuda.synchronize()
+want = step()
+for r in replays:
+    for x, y in zip(r, want):
+        assert torch.equal(x, y)
+cache.check()
+print("ok")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_inside_a_capture():
+    """A fresh process whose first windowed, paged and cache calls are captured: every replay gives the eager results."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL_CAPTURED, os.path.join(root, "hazyresearch_flash-attention_amd")],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split()[-1] == "ok", r.stdout[-2000:] + r.stderr[-4000:]
