@@ -10,12 +10,13 @@
 // l takes P unrounded). Key groups walk every KG-th tile and are joined through LDS at the end; a split walks a
 // contiguous share of the tiles and leaves O, m and l in the workspace for fa_window_join_kernel.
 //
-// What bounds it. Dense: a wave reads a whole K and V tile from LDS for its 32 rows, 128 bytes a cycle and CU, which at
-// head_dim 128 takes as long as the tile's matrix instructions; 32768 tokens, 8 heads of 128 on 2, window 4096: 562 us,
-// 931 TFLOP/s of the 1273 that a large library product reaches here. At head_dim 64 the exponentials and the rest of the
-// softmax take twice the matrix instructions' time (vector units 64 % busy, matrix units 23 %), and short windows the
-// latency of a workgroup's start and end: 8 x 2048 tokens, 12 heads, window 256: 39 us. Paged, few rows: HBM; 64 single
-// tokens over caches of up to 8191, 32 heads of 128 on 8: 232 us, 4.8 TB/s (a copy of 2 GiB: 4.9).
+// What bounds it. Dense, head_dim 128: 32768 tokens, 8 heads on 2, window 4096: 562 us, 931 TFLOP/s of the 1273 that a
+// large library product reaches here; matrix units 52 % busy, vector units 52 %, LDS 27 %, at two waves a SIMD, whose
+// phases hide each other hardly more: one half tile's exponentials placed between the other's products, and priorities
+// for either phase, changed nothing. At head_dim 64 the softmax takes twice the matrix instructions' time (vector units
+// 65 % busy, matrix units 23 %), and short windows the latency of a workgroup's start and end: 8 x 2048 tokens, 12 heads,
+// window 256: 39 us. Paged, few rows: HBM; 64 single tokens over caches of up to 8191, 32 heads of 128 on 8: 232 us,
+// 4.8 TB/s (a copy of 2 GiB: 4.9).
 //
 // Tiles that a wave sees whole take no mask; a tile at the window's edge, the diagonal or the end takes the mask
 // path, as does one with drafted tokens or a page that is not there.
