@@ -57,10 +57,6 @@ SOURCE_FLAGS = {
     # windowed, 8192 tokens, 16 heads of 128 on 4: dQ 120 us for 125, dK and dV 210 for 225; at head_dim 64 it loses (60 for 54)
     "fa_window_d128.hip": _TRACKERS,
 }
-# no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on this part
-_NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-for _src in WINDOW_TUS + ["fa_window_api.cpp", "fa_cache.hip"]:
-    SOURCE_FLAGS[_src] = SOURCE_FLAGS.get(_src, []) + _NO_PACKED_FP32
 ARCH = os.environ.get("FA_OFFLOAD_ARCH", "gfx950")
 
 
@@ -74,6 +70,9 @@ def hipcc():
 def common_flags():
     return ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", INCLUDE, "-I", CSRC,
             "-mllvm", "-amdgpu-mfma-vgpr-form",  # keep MFMA C/D in VGPRs: no accvgpr shuffles
+            # no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on this part (without them
+            # the same bits, and times within 2 %)
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
             "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
 
 
