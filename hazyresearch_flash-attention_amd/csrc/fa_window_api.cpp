@@ -33,6 +33,21 @@ int order_for(int64_t pairs, int64_t window, int64_t max_k, int head_dim) {
     }
     return 2 * keys <= max_k ? 0 : -1;
 }
+int cus() {
+    const int n = device_cus();
+    return n > 0 ? n : 256;
+}
+
+// Whether the products take P and dS in two 16-bit parts (fa_window_fwd_kernel.h, FINE): workgroups of `rows` packed rows
+// that see few keys and all run at once, so that latency and not the matrix units bounds the call, and whose results are few,
+// so that their roundings do not average out. 5 sequences up to 701, 6 heads of 80 on 2, window 100: kernels 77 us for 66,
+// the call 80 either way (the host's); 8 x 2048 tokens, 12 heads of 64, window 100, 1536 workgroups: 175 for 141.
+bool takes_fine(const FaWindowArgs *a, int64_t window, int rows) {
+    const int group = a->nheads / a->nheads_k;
+    const int64_t seen = window + rows / group + 1 + a->num_sinks;
+    const int64_t wgs = ((int64_t)a->max_seqlen_q * group + rows - 1) / rows * a->nheads_k * a->batch;
+    return (seen < a->max_seqlen_k ? seen : a->max_seqlen_k) <= 256 && wgs <= 2 * cus();
+}
 bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // what both entry families ask of the sizes
@@ -169,11 +184,9 @@ PagedPlan plan_paged(const FaPagedArgs *a) {
     }
     const int64_t tiles = (keys + bn - 1) / bn;
     const int64_t base = (int64_t)p.nrb * a->nheads_k * a->batch;
-    int cus = device_cus();
-    if (cus <= 0) cus = 256;
     // workgroups that a CU holds at once (LDS and registers of the shapes, by head-dim tile)
     const int per_cu = (p.shape == WIN_1X4X32 ? 1 : 2) * (tile_of(a->head_dim) == 128 ? 1 : 2);
-    const int64_t slots = (int64_t)cus * per_cu;
+    const int64_t slots = (int64_t)cus() * per_cu;
     int64_t want = 1, best = 0;
     for (int64_t n = 1; n <= 128 && (n == 1 || 2 * kg * n <= tiles); ++n) {
         const int64_t rounds = (base * n + slots - 1) / slots, steps = ((tiles + n - 1) / n + kg - 1) / kg;
@@ -203,6 +216,7 @@ WinBwdPlan plan_bwd(const FaWindowArgs *a, WinBwdArgs &w, char *ws, int64_t &byt
     w.window = (int)window;
     p.order = order_for((int64_t)a->nheads_k * a->batch, window, p.max_k, a->head_dim);
     w.sinks = a->num_sinks < p.max_k ? a->num_sinks : p.max_k;
+    p.fine = takes_fine(a, window, 32 * WIN_DQ_WAVES);
     w.chunks = w.sink_blocks = w.per_chunk = w.slots = 0;
     bytes = a->total_q * a->nheads * (int64_t)sizeof(f32x2);
     bytes = (bytes + 255) / 256 * 256;
@@ -267,6 +281,7 @@ int fa_window_fwd(const FaWindowArgs *a, void *stream) {
     w.dsplit = Div::of(1);
     w.order = BlockOrder::of(w.nrb, w.nheads_k * w.batch, order_for((int64_t)w.nheads_k * w.batch, w.window, a->max_seqlen_k, a->head_dim));
     w.scale = a->softmax_scale;
+    w.fine = takes_fine(a, w.window, 32 * WIN_FWD_WAVES);
     if ((rc = grid_ok("fa_window_fwd", (int64_t)w.nrb * w.nheads_k * w.batch))) return rc;
     hipStream_t s = (hipStream_t)stream;
     hipError_t e;

@@ -69,7 +69,10 @@ struct WinDqCfg {
 // Measured: 8192 tokens, 16 heads of 128 on 4, window 1024: 120 us (matrix units 48 % busy, two waves a SIMD that wait for
 // LDS between products); 8 x 2048 tokens, 12 heads of 64, window 256: 54 us (26 %).
 constexpr int WIN_EXACT_TILES = 4;
-template <int D, typename T, int NW>
+//
+// FINE (small calls, takes_fine in fa_window_api.cpp): dS, and P for dV, go to their products in two 16-bit parts, as
+// in the forward: what their rounding leaves (1.4 and more of a single rounding, where outputs are few) goes to 1.0.
+template <int D, typename T, int NW, bool FINE>
 __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdArgs a) {
     using C = WinDqCfg<D, NW>;
     using S = Swz<D>;
@@ -213,13 +216,19 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
                 for (int r = 0; r < 16; ++r) dsum += s[r];
                 continue;
             }
-            typename T::frag pf[2];
+            typename T::frag pf[2], pl[2];
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 u32x4 pk;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) pk[e] = T::pack2(s[8 * s2 + 2 * e], s[8 * s2 + 2 * e + 1]);
                 pf[s2] = as_frag<T>(pk);
+                if constexpr (FINE) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        pk[e] = T::pack2(s[8 * s2 + 2 * e] - T::lo_float(pk[e]), s[8 * s2 + 2 * e + 1] - T::hi_float(pk[e]));
+                    pl[s2] = as_frag<T>(pk);
+                }
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
@@ -228,7 +237,9 @@ __global__ __launch_bounds__(64 * NW, 2) void fa_window_dq_kernel(const WinBwdAr
                     const int to = ro + 16 * s2 * S::ROW_BYTES;
                     const u32x2 lo = lds_read_tr(kb, t_rd[dt][0] + to);
                     const u32x2 hv = lds_read_tr(kb, t_rd[dt][1] + to);
-                    dq[dt] = T::mfma32(as_frag<T>(u32x4{lo[0], lo[1], hv[0], hv[1]}), pf[s2], dq[dt]);
+                    const auto kt = as_frag<T>(u32x4{lo[0], lo[1], hv[0], hv[1]});
+                    dq[dt] = T::mfma32(kt, pf[s2], dq[dt]);
+                    if constexpr (FINE) dq[dt] = T::mfma32(kt, pl[s2], dq[dt]);
                 }
         }
     };
@@ -338,8 +349,8 @@ __device__ __forceinline__ void dma4(i32x4 srd, int voff, uint32_t lds) {
 //
 // Measured: 8192 tokens, 16 heads of 128 on 4, window 1024, 16 sinks: 210 us (matrix units 36 % busy, LDS 30 %: a step is a
 // chain of two products, the exponentials between them and a barrier); 8 x 2048 tokens, 12 heads of 64, window 256: 69 us.
-template <int D, typename T, int NW, bool PAIR>
-__global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel(const WinBwdArgs a) {
+template <int D, typename T, int NW, bool PAIR, bool FINE>
+__global__ __launch_bounds__(64 * NW, D <= 64 && !FINE ? 3 : 2) void fa_window_dkv_kernel(const WinBwdArgs a) {
     using C = WinDkvCfg<D, NW, PAIR>;
     using S = Swz<D>;
     constexpr float LOG2E = 1.4426950408889634f;
@@ -541,6 +552,19 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
 #pragma unroll
             for (int e = 0; e < 4; ++e) out[sg][e] = T::pack2(x[8 * sg + 2 * e], x[8 * sg + 2 * e + 1]);
     };
+    // acc^T += rows^T b, b packed already; FINE: and what the packing left of it
+    auto add_product = [&](f32x16 (&acc)[D / 32], int rows, const f32x16 &b, const u32x4 (&bv)[2]) __attribute__((always_inline)) {
+        add_t(acc, rows, bv);
+        if constexpr (FINE) {
+            u32x4 rest[2];
+#pragma unroll
+            for (int sg = 0; sg < 2; ++sg)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    rest[sg][e] = T::pack2(b[8 * sg + 2 * e] - T::lo_float(bv[sg][e]), b[8 * sg + 2 * e + 1] - T::hi_float(bv[sg][e]));
+            add_t(acc, rows, rest);
+        }
+    };
     // the tile's rows as A operands, all on their way before the first is used
     auto read_rows = [&](int rows, u32x4 (&x)[D / 16]) __attribute__((always_inline)) {
 #pragma unroll
@@ -601,8 +625,8 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         pack(s, pk);
         pack(dp, sk);
         if constexpr (!PAIR) {
-            add_t(dv, buf + C::TILE, pk);
-            add_t(dk, buf, sk);
+            add_product(dv, buf + C::TILE, s, pk);
+            add_product(dk, buf, dp, sk);
         }
     };
     // PAIR: S of a tile (P wave) or dP (dS wave), started one step before the rest of its work, so that the matrix
@@ -629,7 +653,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
             *reinterpret_cast<f32x4 *>(img + (q4 * 64 + lane) * 16) = f32x4{s[4 * q4], s[4 * q4 + 1], s[4 * q4 + 2], s[4 * q4 + 3]};
         u32x4 pk[2];
         pack(s, pk);
-        add_t(dk, buf + C::TILE, pk);                  // dV^T
+        add_product(dk, buf + C::TILE, s, pk);         // dV^T
     };
     auto first_ds = [&](int buf, f32x16 &dp) __attribute__((always_inline)) {
         u32x4 y[D / 16];
@@ -653,7 +677,7 @@ __global__ __launch_bounds__(64 * NW, D <= 64 ? 3 : 2) void fa_window_dkv_kernel
         }
         u32x4 sk[2];
         pack(dp, sk);
-        add_t(dk, buf, sk);                            // dK^T
+        add_product(dk, buf, dp, sk);                  // dK^T
     };
 
     // ---- the walk

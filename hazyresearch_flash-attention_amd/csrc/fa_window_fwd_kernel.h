@@ -6,8 +6,8 @@
 // A workgroup has NWR row waves (32 packed rows each, fa_window_common.h) times KG key groups. Tiles of BN keys
 // go HBM -> LDS by LDS-DMA into two buffers per key group; the scores are computed swapped (S^T = K Q^T), so a
 // lane owns a row: its mask is one 32-bit word per 32 keys, its max and sum need one lane exchange per tile, and
-// P feeds O^T += V^T P^T from registers (rounded to 16 bits: the operand type of the matrix instruction; the sum
-// l takes P unrounded). Key groups walk every KG-th tile and are joined through LDS at the end; a split walks a
+// P feeds O^T += V^T P^T from registers (rounded to 16 bits, the operand type of the matrix instruction, or in two
+// such parts, see FINE; the sum l takes P unrounded). Key groups walk every KG-th tile and are joined through LDS at the end; a split walks a
 // contiguous share of the tiles and leaves O, m and l in the workspace for fa_window_join_kernel.
 //
 // What bounds it. Dense, head_dim 128: 32768 tokens, 8 heads on 2, window 4096: 562 us, 931 TFLOP/s of the 1273 that a
@@ -40,6 +40,7 @@ struct WinFwdArgs {
     int batch, nheads, nheads_k, head_dim, group;
     int num_pages, page_shift, num_seqs, max_blocks, tree_words;
     int max_q, lse_stride, window, sinks, nrb, nsplit;
+    int fine;                     // dense: which of the two kernels
     float scale;
     Div dgroup, dheads, dsplit;   // by group, nheads_k, nsplit
     BlockOrder order;             // dense; paged: its blk divides by nrb
@@ -71,7 +72,12 @@ struct WinFwdCfg {
 // rarely rescaled. The same relative rounding, and fp16's smallest P is 2^8 times nearer to the row's largest.
 constexpr float WIN_RESCALE = 8.0f;
 
-template <int D, typename T, int NWR, int KG, int BN, bool PAGED, bool TREE>
+//
+// FINE: P goes to the product in two 16-bit parts, what the first leaves in the second, with half as many matrix
+// instructions more. Rounded once, P brings as much error as the rounding of the output (rms, together 1.41 of it);
+// so 1.0. Taken where it costs nothing or little: few rows over a cache (HBM or latency bounds them: 64 single
+// tokens over caches of up to 8191 take 235 us for 233) and small dense calls (takes_fine, fa_window_api.cpp).
+template <int D, typename T, int NWR, int KG, int BN, bool PAGED, bool TREE, bool FINE>
 __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinFwdArgs a) {
     using C = WinFwdCfg<D, NWR, KG, BN>;
     using S = Swz<D>;
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
                 for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
         }
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        typename T::frag pf[C::NS][2];
+        typename T::frag pf[C::NS][2], pl[FINE ? C::NS : 1][2];
 #pragma unroll
         for (int st = 0; st < C::NS; ++st) {
 #pragma unroll
@@ -416,6 +422,12 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
 #pragma unroll
                 for (int e = 0; e < 4; ++e) pk[e] = T::pack2(s[st][8 * s2 + 2 * e], s[st][8 * s2 + 2 * e + 1]);
                 pf[st][s2] = as_frag<T>(pk);
+                if constexpr (FINE) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        pk[e] = T::pack2(s[st][8 * s2 + 2 * e] - T::lo_float(pk[e]), s[st][8 * s2 + 2 * e + 1] - T::hi_float(pk[e]));
+                    pl[st][s2] = as_frag<T>(pk);
+                }
             }
         }
         l_i += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -427,7 +439,9 @@ __global__ __launch_bounds__(64 * NWR * KG) void fa_window_fwd_kernel(const WinF
                 for (int s2 = 0; s2 < 2; ++s2) {
                     const u32x2 lo = lds_read_tr(vb, v_rd[dt][st][s2][0]);
                     const u32x2 hv = lds_read_tr(vb, v_rd[dt][st][s2][1]);
-                    o[dt] = T::mfma32(as_frag<T>(u32x4{lo[0], lo[1], hv[0], hv[1]}), pf[st][s2], o[dt]);
+                    const auto vt = as_frag<T>(u32x4{lo[0], lo[1], hv[0], hv[1]});
+                    o[dt] = T::mfma32(vt, pf[st][s2], o[dt]);
+                    if constexpr (FINE) o[dt] = T::mfma32(vt, pl[FINE ? st : 0][s2], o[dt]);
                 }
     };
 

@@ -22,6 +22,7 @@ constexpr int WIN_DQ_WAVES = 4, WIN_DKV_BLOCKS = 4;
 constexpr int win_dkv_waves(int D) { return D == 128 ? 2 * WIN_DKV_BLOCKS : WIN_DKV_BLOCKS; }
 struct WinBwdPlan {
     int max_rows, max_k, order;
+    bool fine;
 };
 template <int D> hipError_t launch_window_bwd(const WinBwdArgs &a, int dtype, const WinBwdPlan &p, hipStream_t s);
 // the error text of the C ABI (fa_api.cpp)

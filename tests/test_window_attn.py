@@ -399,6 +399,31 @@ def test_refusals_on_the_gpu():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_small_calls_round_once(dtype, d):
+    """A small call with a short window takes P and dS in two parts: its errors (rms) are those of one rounding, half a
+    step at most and uniform over it, against the 1.4 of a second rounding; the same rows in a batch too large for it
+    keep the bounds that count both."""
+    from window_testutil import check, cu, dense_reference, randn
+    n, many = 200, 200
+    q, k, v, dout = (randn(i, (n, 2, d), dtype) for i in range(4))
+    r, _, e = dense_reference(q, k, v, [n], [n], 30, 2, d ** -0.5, dtype, dout)
+    for copies in (1, many):
+        x = [t.repeat(copies, 1, 1).requires_grad_() for t in (q, k, v)]
+        c = cu([n] * copies)
+        out = _func()(*x, c, c, n, n, 30, 2)
+        grads = torch.autograd.grad(out, x, dout.repeat(copies, 1, 1))
+        for name, got in zip(("out", "dq", "dk", "dv"), (out.detach(), *grads)):
+            got = got[-n:]
+            check(name, got, r[name], e[name])
+            if copies == 1:
+                rounded = r[name].to(dtype).double()
+                rms = lambda a: (a - r[name]).pow(2).mean().sqrt()
+                assert rms(got.double()) <= 1.1 * rms(rounded)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
 @pytest.mark.parametrize("most", [0, 1, 10, 40])
 def test_rows_past_max_seqlen_are_left_alone(d, most):
     """Sequences longer than max_seqlen_q says (C ABI): what is asked for is right, nothing else is written, the rows
