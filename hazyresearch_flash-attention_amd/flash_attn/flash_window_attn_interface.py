@@ -10,7 +10,8 @@ A row with p < 0 sees nothing: its output and its gradient are 0, its lse -inf. 
 sequence belong to none: output and gradients are 0 there.
 
 Scores, softmax statistics and sums are fp32; the probabilities are rounded to the input type for the product with
-v (and dS for those with q and k), as they are in the other kernels. Results do not depend on the order in which
+v (and dS for those with q and k), as they are in the other kernels; small calls with short windows take them in two such
+parts, so that the output's own rounding is all that is left. Results do not depend on the order in which
 workgroups run: there are no atomics, gradients of shared key/value heads included.
 """
 from flash_attn import flash_attn_hip as _hip
